@@ -1,0 +1,232 @@
+"""Causal attention inside the documents of packed rows, forward and backward.
+
+The kernels behind `Runtime.attention = "documents"`, beside the library call of kernels/attention.py (58-93 of the
+reference). Documents need not tile the rows and nothing is gathered: a plan, made once per batch and shared by all
+layers and by checkpoint replays, lists the tiles of every document, longest work first.
+
+    y      = softmax(scale * q k^T, keys of the same document up to the query) v       zeros outside documents
+    dv     = P^T dy,   dS = P * (dy v^T - sum(dy * y)),   dq = scale dS k,   dk = scale dS^T q
+
+The backward pass recomputes P from q, k and the row's log-sum. Every sum has a fixed order: the query gradients are one
+kernel, the key and value gradients another whose pieces are added in plan order, so repeated calls agree bit for bit.
+bf16 and fp16 run on the tensor cores; fp32, and operands whose rows are not 16-byte aligned, on FMA units.
+A NaN or infinity outside the documents reaches nothing; one inside a document reaches that document only.
+"""
+
+import ctypes
+from dataclasses import dataclass, field
+
+import numpy
+import torch
+
+from .. import _lib
+
+KEY_TILE = 128              # keys of one piece of the key-gradient pass (include/ct_b200.h)
+_PIECES_PER_SM, _SMS, _SMALLEST_PIECE = 4, 148, 16
+
+
+@dataclass(frozen=True)
+class DocumentPlan:
+    """Tiles of the documents of one batch, for one number of heads. Made by `prepare_documents`."""
+    shape: tuple                    # (rows, width)
+    heads: int
+    kv_heads: int
+    spans: tuple
+    table: torch.Tensor             # int32 [records, 4] on the device
+    sections: tuple                 # ((first record, count), ...) of the six sections
+    key_slots: int
+    host_sections: ctypes.Array = field(repr=False, compare=False, default=None)
+
+
+def _tiles(starts, lengths, step):
+    """(document, first token) of every tile of `step` tokens."""
+    counts = -(-lengths // step)
+    document = numpy.repeat(numpy.arange(len(lengths)), counts)
+    first = numpy.arange(len(document)) - numpy.repeat(numpy.cumsum(counts) - counts, counts)
+    return document, first * step
+
+
+def _query_section(starts, lengths, step):
+    document, first = _tiles(starts, lengths, step)
+    keys = numpy.minimum(first + step, lengths[document])       # a query tile's work: the keys it sees
+    order = numpy.argsort(-keys, kind="stable")
+    document, first = document[order], first[order]
+    return numpy.stack((starts[document], lengths[document], first, numpy.zeros_like(first)), 1)
+
+
+def _key_sections(starts, lengths, tile_tokens, head_blocks, kv_heads):
+    """Pieces of the key tiles and the sums over them. A key tile's queries are all later tokens of the document, so the
+    work of the tiles differs by the document's length: tiles are cut into pieces of at most a fraction of an SM's share
+    (but no smaller than _SMALLEST_PIECE query tiles, whose cost covers that of writing and adding a share)."""
+    document, first_key = _tiles(starts, lengths, KEY_TILE)
+    work = -(-(lengths[document] - first_key) // tile_tokens) * head_blocks
+    largest = max(_SMALLEST_PIECE, -(-int(work.sum()) * kv_heads // (_SMS * _PIECES_PER_SM)))
+    pieces = -(-work // largest)
+    tile = numpy.repeat(numpy.arange(len(work)), pieces)
+    index = numpy.arange(len(tile)) - numpy.repeat(numpy.cumsum(pieces) - pieces, pieces)
+    first, last = work[tile] * index // pieces[tile], work[tile] * (index + 1) // pieces[tile]
+    split = pieces > 1
+    slots = numpy.where(split, pieces, 0)
+    first_slot = numpy.cumsum(slots) - slots
+    slot = numpy.where(split[tile], first_slot[tile] + index, -1)
+    order = numpy.argsort(-(last - first), kind="stable")
+    zero = numpy.zeros_like(tile)
+    records = numpy.stack((starts[document][tile], lengths[document][tile], first_key[tile], slot, first, last, zero, zero), 1)
+    rows = numpy.minimum(KEY_TILE, lengths[document] - first_key)
+    sums = numpy.stack((starts[document] + first_key, rows, first_slot, slots), 1)[split]
+    return records[order].reshape(-1, 4), sums, int(slots.sum())
+
+
+def prepare_documents(shape, spans, device, heads, kv_heads=1):
+    """The plan of a [rows, width] batch whose documents are `spans`, ((row, start, end), ...) as `segments.runs` gives
+    them: any order, gaps allowed, no token in two documents."""
+    rows, width = (int(n) for n in shape)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
+    spans = tuple(spans)
+    table = numpy.array(spans, dtype=numpy.int64).reshape(len(spans), 3)
+    row, start, end = table[:, 0], table[:, 1], table[:, 2]
+    if ((row < 0) | (row >= rows) | (start < 0) | (end < start) | (end > width)).any():
+        raise ValueError("a document span lies outside the batch")
+    if rows * width >= 2 ** 31 - 256:
+        raise NotImplementedError(f"{rows * width} tokens in one batch")
+    starts, lengths = row * width + start, end - start
+    starts, lengths = starts[lengths > 0], lengths[lengths > 0]
+    order = numpy.argsort(starts, kind="stable")
+    starts, lengths = starts[order], lengths[order]
+    ends = starts + lengths
+    if (starts[1:] < ends[:-1]).any():
+        raise ValueError("document spans overlap")
+    tile_tokens = _lib.load().ct_attention_tile_tokens(heads, kv_heads)
+    head_blocks = heads // kv_heads * tile_tokens // 128
+    keys, sums, slots = _key_sections(starts, lengths, tile_tokens, head_blocks, kv_heads)
+    gap_start = numpy.concatenate(([0], ends))
+    gap_length = numpy.concatenate((starts, [rows * width])) - gap_start
+    gap_start, gap_length = gap_start[gap_length > 0], gap_length[gap_length > 0]
+    run, offset = _tiles(gap_start, gap_length, 64)
+    zero = numpy.zeros_like(offset)
+    gaps = numpy.stack((gap_start[run] + offset, numpy.minimum(64, gap_length[run] - offset), zero, zero), 1)
+    parts = (_query_section(starts, lengths, 2 * tile_tokens), _query_section(starts, lengths, tile_tokens), keys, sums,
+             _query_section(starts, lengths, KEY_TILE), gaps)
+    first = numpy.cumsum([0] + [len(part) for part in parts])
+    sections = tuple((int(first[i]), len(part) // 2 if i == 2 else len(part)) for i, part in enumerate(parts))
+    records = numpy.ascontiguousarray(numpy.concatenate(parts), dtype=numpy.int32)
+    host = (ctypes.c_int64 * 12)(*(n for pair in sections for n in pair))
+    return DocumentPlan((rows, width), heads, kv_heads, spans, torch.from_numpy(records).to(device), sections, slots, host)
+
+
+def _check(q, k, v, plan):
+    _lib.require_cuda(q, k, v)
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError("document attention takes q [rows, width, heads, head_dim] and k, v [rows, width, kv_heads, head_dim]")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise TypeError("q, k and v must have one dtype")
+    _lib.code_of(q.dtype)
+    if not q.device == k.device == v.device == plan.table.device:
+        raise ValueError("q, k, v and the plan must be on one device")
+    if tuple(q.shape[:2]) != plan.shape or q.shape[2] != plan.heads or k.shape[2] != plan.kv_heads:
+        raise ValueError(f"the plan is for a batch of {plan.shape} tokens with {plan.heads} / {plan.kv_heads} heads")
+    if q.shape[3] > 128:
+        raise NotImplementedError(f"head_dim {q.shape[3]} is above 128")
+
+
+def _rows(tensor):
+    """The tensor as [tokens, heads, head_dim] with contiguous channels, copied only where the strides demand it."""
+    flat = tensor.flatten(0, 1)
+    if flat.stride(2) != 1 and flat.shape[2] > 1 or any(s <= 0 for s, n in zip(flat.stride(), flat.shape) if n > 1):
+        flat = flat.contiguous()
+    return flat
+
+
+def _operands(*tensors):
+    """(pointer, token stride, head stride) of each; the strides of dimensions of one element are made regular."""
+    result = []
+    for tensor in tensors:
+        tokens, heads, dim = tensor.shape
+        head_stride = tensor.stride(1) if heads > 1 else dim
+        token_stride = tensor.stride(0) if tokens > 1 else heads * head_stride
+        result += [tensor.data_ptr(), token_stride, head_stride]
+    return result
+
+
+def _aligned(tensor):
+    """A contiguous form whose first element is 16-byte aligned."""
+    tensor = tensor.contiguous()
+    return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
+
+
+def attention_forward(q, k, v, plan, *, scale=None, keep_lse=True):
+    """(y, lse): the attention output, shaped like q, and the rows' base-2 log-sums [tokens, heads] (None without
+    `keep_lse`). `scale` defaults to head_dim ** -0.5."""
+    _check(q, k, v, plan)
+    rows = [_rows(t) for t in (q, k, v)]
+    tokens, heads, dim = rows[0].shape
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty((tokens, heads), device=q.device, dtype=torch.float32) if keep_lse else None
+    if out.numel() == 0:
+        return out, lse
+    library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q):
+        path = _path(library, operands, heads, plan.kv_heads, dim, code)
+        _lib.check(library.ct_attention_forward(
+            *operands, out.data_ptr(), _lib.pointer(lse), plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads,
+            dim, scale, code, path, _lib.stream_of(q)))
+    return out, lse
+
+
+def _path(library, operands, heads, kv_heads, dim, code):
+    if _lib.gemm_path == _lib.PATH_SIMT:
+        return _lib.PATH_SIMT
+    return library.ct_attention_path(*operands, heads, kv_heads, dim, code)
+
+
+def attention_backward(dy, q, k, v, y, lse, plan, *, scale=None):
+    """(dq, dk, dv) from the upstream gradient `dy` of `y` and what `attention_forward` returned."""
+    _check(q, k, v, plan)
+    if dy.shape != q.shape or y.shape != q.shape:
+        raise ValueError("dy and y must be shaped like q")
+    if dy.device != q.device or y.device != q.device or lse.device != q.device:
+        raise ValueError("dy, y and lse must be on the device of q")
+    if lse.shape != (q.shape[0] * q.shape[1], q.shape[2]) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be the contiguous fp32 [tokens, heads] of the forward pass")
+    rows = [_rows(t) for t in (q, k, v)]
+    dy, y = _aligned(dy.to(q.dtype)), _aligned(y.to(q.dtype))
+    tokens, heads, dim = rows[0].shape
+    dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+    if dq.numel() == 0:
+        return dq, dk, dv
+    library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q):
+        path = _path(library, operands, heads, plan.kv_heads, dim, code)
+        size = library.ct_attention_backward_workspace(tokens, heads, plan.kv_heads, dim, plan.key_slots, path)
+        workspace = torch.empty(size, device=q.device, dtype=torch.uint8)
+        _lib.check(library.ct_attention_backward(
+            *operands, y.data_ptr(), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads, dim, scale, code, path, workspace.data_ptr(),
+            _lib.stream_of(q)))
+    return dq, dk, dv
+
+
+class DocumentAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, plan, scale):
+        keep = any(ctx.needs_input_grad[:3])
+        y, lse = attention_forward(q, k, v, plan, scale=scale, keep_lse=keep)
+        ctx.plan, ctx.scale = plan, scale
+        if keep:
+            ctx.save_for_backward(q, k, v, y, lse)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, k, v, y, lse = ctx.saved_tensors
+        return (*attention_backward(dy, q, k, v, y, lse, ctx.plan, scale=ctx.scale), None, None)
+
+
+def document_attention(q, k, v, plan, *, scale=None):
+    """Causal attention inside the plan's documents: q [rows, width, heads, head_dim], k and v
+    [rows, width, kv_heads, head_dim] -> shaped like q, differentiable in all three."""
+    return DocumentAttention.apply(q, k, v, plan, scale)

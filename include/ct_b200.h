@@ -467,6 +467,47 @@ CT_API int ct_adamw_update(int count, void* const* grads, void* const* params, v
                            const float* divisor, const float* norm, float lr, float beta1, float beta2,
                            float eps, int64_t step, int write_grads, void* stream);
 
+/* ---- document attention ----------------------------------------------------------
+ * Stand beside the library call of kernels/attention.py:58-93 of the reference (flash_dense): causal attention inside every document
+ * of a batch of packed rows, forward and backward, for documents that need not tile the batch.
+ *   q [tokens, heads, head_dim], k / v [tokens, kv_heads, head_dim] with a token and a head stride in elements and
+ *   contiguous channels; head h reads key head h / (heads / kv_heads); head_dim <= 128.
+ *   y = softmax(scale * q k^T over the keys of the same document up to the query) v, zeros for tokens of no document;
+ *   lse [tokens, heads] fp32 (may be null in a pass without gradients) = log2 of the sum of exp(scaled scores); rows of
+ *   no document are not written.
+ *   backward recomputes the probabilities from q, k and lse; dq, dk, dv are zero for tokens of no document.
+ *   out, dy, dq [tokens, heads, head_dim] and dk, dv [tokens, kv_heads, head_dim] are contiguous.
+ * `plan` (device) is a table of records of four int32 (document's first token, document's length, a, b), in sections;
+ * `sections` (HOST) is six pairs (first record, count):
+ *   0 forward: query tiles of 2 * tile_tokens tokens, a = first token inside the document
+ *   1 query gradients: query tiles of tile_tokens tokens, a = first token
+ *   2 key gradients: pieces of 128-key tiles, two records each - (start, length, a = first key, b = slot or -1) and
+ *     (first, last, 0, 0): query tiles [first, last) of the ceil((length - a) / tile_tokens) tiles from token a on, taken
+ *     for each of the group's head blocks in turn; a piece with a slot writes its share to the workspace
+ *   3 sums of the pieces: (first token, rows, first slot, slots)
+ *   4 tiles of 128 tokens for the shape-generic kernels, a = first token
+ *   5 runs of tokens of no document: (first token, count, 0, 0)
+ * with tile_tokens = ct_attention_tile_tokens(heads, kv_heads). Every record must lie inside the batch: the table is
+ * trusted (causal_tuner_b200.kernels.attention_cuda.prepare_documents builds it).
+ * `path` is CT_PATH_TCGEN05 or CT_PATH_SIMT, as ct_attention_path answers for the operands; out, dy and the gradients
+ * are 16-byte aligned for the former. Sums have a fixed order on both: repeated calls are bit-identical.
+ * `key_slots` = the number of slots that section 2 names. */
+CT_API int ct_attention_tile_tokens(int heads, int kv_heads);
+CT_API int ct_attention_path(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                             int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int heads, int kv_heads,
+                             int head_dim, int dtype);
+CT_API int ct_attention_forward(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                                int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* out, float* lse,
+                                const int32_t* plan, const int64_t* sections, int64_t tokens, int heads, int kv_heads,
+                                int head_dim, float scale, int dtype, int path, void* stream);
+CT_API int64_t ct_attention_backward_workspace(int64_t tokens, int heads, int kv_heads, int head_dim, int64_t key_slots,
+                                               int path);
+CT_API int ct_attention_backward(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
+                                 int64_t k_head, const void* v, int64_t v_token, int64_t v_head, const void* out,
+                                 const float* lse, const void* dy, void* dq, void* dk, void* dv, const int32_t* plan,
+                                 const int64_t* sections, int64_t tokens, int heads, int kv_heads, int head_dim,
+                                 float scale, int dtype, int path, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
