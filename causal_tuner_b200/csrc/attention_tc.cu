@@ -1,7 +1,1068 @@
+// Document attention on the Blackwell tensor cores (tcgen05 + TMEM + TMA), bf16 and fp16, head_dim a multiple of 8 up
+// to 128.
+//
+// Rows of a tile. The query heads of a group read the same keys, so a 128-row tile holds 128 / P tokens x P heads (P =
+// the largest power of two that divides the group, packed_heads): with 32 heads on one key head a tile is 4 tokens, a
+// 64-token document fills 16 tiles instead of half-filling 32, and both 128-row stages of a CTA end on the same key
+// tile. One TMA box {64 channels, P heads, 128 / P tokens} brings such a tile in the 128-byte swizzle the tensor core
+// reads; K and V tiles are boxes of 128 keys, each serving as a K-major operand (scores) and as an MN-major one.
+//
+// head_dim below 64 or 128 is padded by the copies themselves (channels past the tensor are zeros).
+// Rows of another document that a tile takes in: scores are dropped by the key limit of each row, and operand rows that
+// would be MULTIPLIED by a zero probability are overwritten with zeros in shared memory, so that a NaN in foreign or
+// padding rows cannot spread.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "attention.cuh"
+#include "tcgen05.cuh"
+
 namespace ct {
-bool attention_tc_supported(const AttentionArgs&) { return false; }
-int attention_tc_forward(const AttentionArgs&, cudaStream_t) { return fail(CT_ERR_UNSUPPORTED, "attention_tc"); }
-int64_t attention_tc_workspace(int64_t, int, int) { return 0; }
-int attention_tc_backward(const AttentionArgs&, cudaStream_t) { return fail(CT_ERR_UNSUPPORTED, "attention_tc"); }
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int KEYS = 128;                          // keys per tile
+constexpr uint32_t BOX_BYTES = 128 * 128;          // 128 rows x 64 channels
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {   // special-function unit, relative error about 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// D += A . B with A in shared memory (K-major) or in TMEM (packed pairs along k), B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  umma_bf16(d, a_lo, desc_high(1024), b_lo, b_hi, idesc, accumulate);
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
+      ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: fp32 accumulator, both operands T, A K-major, M = 128.
+template <typename T> __device__ __forceinline__ uint32_t operand_desc(bool b_mn, int n) {
+  const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+
+// scores: D[128, n] = A[128, HD] . B[n, HD]^T, both tiles as 128-row boxes of 64 channels
+template <typename T, int HD>
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, int n) {
+  const uint32_t idesc = operand_desc<T>(false, n);
+#pragma unroll
+  for (int k = 0; k < HD / 16; ++k) {
+    const uint32_t offset = (k / 4) * BOX_BYTES + (k % 4) * 32;
+    mma_ss(d, desc_low(a + offset, 16), desc_low(b + offset, 16), desc_high(1024), idesc, k > 0);
+  }
+}
+
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t* r) {
+  tmem_store_16(taddr, r);
+  tmem_store_16(taddr + 16, r + 16);
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_alloc(uint32_t slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(512) : "memory");
+}
+
+// Zeros over rows [from, to) of a tile of BOXES boxes, by `threads` threads of which this is number `thread`, made
+// visible to the tensor core.
+template <int BOXES>
+__device__ __forceinline__ void clear_rows(uint32_t tile, int from, int to, int thread, int threads) {
+  for (int i = thread; i < (to - from) * 8 * BOXES; i += threads) {
+    const int row = from + i / (8 * BOXES), piece = i % (8 * BOXES);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (piece / 8) * BOX_BYTES + row * 128 + (piece % 8) * 16), "r"(0)
+                 : "memory");
+  }
+  fence_async_shared();
+}
+
+struct AttentionParams {
+  CUtensorMap q, k, v, dy;
+  const PlanRecord* items;
+  void* out;               // forward: y; backward: dq
+  void* dk;
+  void* dv;
+  float* lse;
+  float* delta;
+  float* partials;
+  int heads, kv_heads, dim;
+  int packed, tile_tokens; // packed * tile_tokens = 128
+  int head_blocks;         // 128-row blocks of heads: heads / packed
+  float scale;
+  int* error_flag;
+};
+
+// The waiting side of the barriers of one CTA (bounded, see tcgen05.cuh).
+struct Waiter {
+  volatile int* abort_flag;
+  int* error_flag;
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, int code) const {
+    return mbar_wait_until(bar, parity, abort_flag, error_flag, code, kWaitLimitNs);
+  }
+};
+
+// A CTA that gave up leaves copies in flight; it stays until they have landed (a bounded pause, no one waits on it).
+__device__ __forceinline__ void settle(const volatile int* abort_flag) {
+  if (!*abort_flag) return;
+  const uint64_t start = global_timer_ns();
+  while (global_timer_ns() - start < 1000000ull) __nanosleep(1000);
+}
+
+// ---- forward -------------------------------------------------------------------------
+// Two 128-row stages per CTA against one stream of key tiles; per stage and tile
+//   tensor core   S = Q K^T (128 x 128), then O += P V with P as the TMEM operand over S's own columns
+//   warpgroup     row maximum and exponentials of S (a thread owns a row), P back to TMEM
+// so one stage's products run under the other's exponentials. O stays in TMEM; it is rescaled by the warpgroup only
+// when a row's maximum has grown by more than 2^8 (P and the sums stay below 2^8 times their scaled size: no
+// overflow in fp32 or fp16, and the final division cancels the factor).
+template <int HD> struct ForwardShape {
+  static constexpr int kBoxes = HD / 64;
+  static constexpr uint32_t kTile = kBoxes * BOX_BYTES;
+  static constexpr int kRing = 2;
+  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + 1024 + 256;
+};
+// Three warpgroups: two own a stage each, the third holds the copy and the MMA warp (two of its warps idle). Launched
+// with 168 registers a thread; the third hands down registers so that a thread can hold a row of 128 scores:
+// 2 x 200 + 104 = 3 x 168.
+constexpr int kForwardThreads = 384;
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr uint32_t kOutColumn = 256;       // TMEM: S of the stages at 0 and 128, O at 256 and 384
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kernel(const __grid_constant__ AttentionParams p) {
+  using Shape = ForwardShape<HD>;
+  constexpr int BOXES = Shape::kBoxes, RING = Shape::kRing;
+  constexpr uint32_t TILE = Shape::kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_tile = smem_u32(smem), k_ring = q_tile + 2 * TILE, v_ring = k_ring + RING * TILE;
+  const uint32_t bars = v_ring + RING * TILE;
+  auto q_full = [&](int s) { return bars + 8u * s; };
+  auto s_full = [&](int s) { return bars + 16u + 8u * s; };
+  auto p_full = [&](int s) { return bars + 32u + 8u * s; };
+  auto o_full = [&](int s) { return bars + 48u + 8u * s; };
+  auto k_full = [&](int r) { return bars + 64u + 8u * r; };
+  auto k_empty = [&](int r) { return bars + 64u + 8u * (RING + r); };
+  auto v_full = [&](int r) { return bars + 64u + 8u * (2 * RING + r); };
+  auto v_empty = [&](int r) { return bars + 64u + 8u * (3 * RING + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 64 + 32 * RING);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(q_full(s), 1);
+      mbar_init(s_full(s), 1);
+      mbar_init(p_full(s), 4);
+      mbar_init(o_full(s), 1);
+    }
+    for (int r = 0; r < RING; ++r) {
+      mbar_init(k_full(r), 1);
+      mbar_init(k_empty(r), 1);
+      mbar_init(v_full(r), 1);
+      mbar_init(v_empty(r), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(tmem_slot));
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Waiter wait{abort_flag, p.error_flag};
+
+  const PlanRecord item = p.items[blockIdx.x / p.head_blocks];
+  const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
+  const int shared = head0 / (p.heads / p.kv_heads);
+  // stage s holds the tokens from item.a + s * tile_tokens; keys [0, end[s]) are all it can see
+  const int first1 = item.a + p.tile_tokens;
+  const int end0 = min(item.length, first1);
+  const int end1 = first1 < item.length ? min(item.length, first1 + p.tile_tokens) : 0;
+  const int n0 = (end0 + KEYS - 1) / KEYS, n1 = (end1 + KEYS - 1) / KEYS;
+  const int n = max(n0, n1);
+  // keys of tile j that stage needs, in steps of 32 columns
+  auto columns = [](int end, int j) { return min(KEYS, (end - j * KEYS + 31) & ~31); };
+
+  if (warp >= 8) {
+   registers_down<104>();
+   if (warp == 8) {
+    if (lane == 0) {
+      for (int j = 0; j < n; ++j) {
+        const int r = j % RING;
+        const uint32_t free_parity = ((j / RING) & 1) ^ 1;
+        if (j == 0) {
+          for (int s = 0; s < (n1 ? 2 : 1); ++s) {
+            mbar_expect_tx(q_full(s), TILE);
+            for (int b = 0; b < BOXES; ++b)
+              tma_load_3d(q_tile + s * TILE + b * BOX_BYTES, &p.q, q_full(s), 64 * b, head0, item.start + item.a + s * p.tile_tokens);
+            if (s == 0) {
+              mbar_expect_tx(k_full(0), TILE);
+              for (int b = 0; b < BOXES; ++b)
+                tma_load_3d(k_ring + b * BOX_BYTES, &p.k, k_full(0), 64 * b, shared, item.start);
+            }
+          }
+        } else {
+          if (!wait(k_empty(r), free_parity, 6)) break;
+          mbar_expect_tx(k_full(r), TILE);
+          for (int b = 0; b < BOXES; ++b)
+            tma_load_3d(k_ring + r * TILE + b * BOX_BYTES, &p.k, k_full(r), 64 * b, shared, item.start + j * KEYS);
+        }
+        if (!wait(v_empty(r), free_parity, 6)) break;
+        mbar_expect_tx(v_full(r), TILE);
+        for (int b = 0; b < BOXES; ++b)
+          tma_load_3d(v_ring + r * TILE + b * BOX_BYTES, &p.v, v_full(r), 64 * b, shared, item.start + j * KEYS);
+      }
+    }
+    __syncwarp();
+   } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t value_desc = desc_high(1024);
+      auto scores = [&](int s, int j) {
+        product_nt<T, HD>(tmem + s * 128, q_tile + s * TILE, k_ring + (j % RING) * TILE, columns(s ? end1 : end0, j));
+        umma_commit(s_full(s));
+      };
+      bool alive = wait(q_full(0), 0, 7) && wait(k_full(0), 0, 7);
+      if (alive) {
+        tcgen05_fence_after();
+        scores(0, 0);
+        if (n1) {
+          alive = wait(q_full(1), 0, 7);
+          if (alive) scores(1, 0);
+        }
+        umma_commit(k_empty(0));
+      }
+      for (int j = 0; j < n && alive; ++j) {
+        const int r = j % RING, next = (j + 1) % RING;
+        if (!wait(v_full(r), (j / RING) & 1, 7)) break;
+        for (int s = 0; s < 2; ++s) {
+          const int count = s ? n1 : n0, end = s ? end1 : end0;
+          if (j < count) {
+            if (!wait(p_full(s), j & 1, 7)) { alive = false; break; }
+            tcgen05_fence_after();
+            const uint32_t idesc = operand_desc<T>(true, HD);
+            const int steps = columns(end, j) / 16;
+            for (int k = 0; k < steps; ++k)
+              mma_ts(tmem + kOutColumn + s * 128, tmem + s * 128 + 8 * k, desc_low(v_ring + r * TILE + k * 2048, BOX_BYTES), value_desc,
+                     idesc, j > 0 || k > 0);
+            if (j + 1 == count) umma_commit(o_full(s));
+          }
+          if (s == 1) umma_commit(v_empty(r));
+          if (j + 1 < n && s == 0 && !wait(k_full(next), ((j + 1) / RING) & 1, 7)) { alive = false; break; }
+          if (j + 1 < count) scores(s, j + 1);
+          if (s == 1 && j + 1 < n) umma_commit(k_empty(next));
+        }
+      }
+    }
+    __syncwarp();
+   }
+  } else {
+    registers_up<200>();
+    const int s = warp >> 2, thread = threadIdx.x & 127;
+    const int count = s ? n1 : n0, end = s ? end1 : end0;
+    const int first = item.a + s * p.tile_tokens;              // the stage's first token
+    const int token = first + thread / p.packed, head = head0 + thread % p.packed;
+    const int last_key = min(token, item.length - 1);
+    const bool negative = p.scale < 0.0f;
+    const float c = fabsf(p.scale) * kLog2e;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;          // this warp's 32 TMEM lanes
+    const uint32_t s_addr = tmem + lanes + s * 128, o_addr = tmem + lanes + kOutColumn + s * 128;
+    // fp16: probabilities are kept 2^7 above their size (at most 2^15 with the late rescaling), so that small ones do not
+    // fall among the subnormals; the sum carries the factor too
+    constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+    float top = -INFINITY, sum = 0.0f;
+    bool alive = true;
+    for (int j = 0; j < count; ++j) {
+      const int cols = columns(end, j);
+      if (!__all_sync(0xffffffffu, wait(s_full(s), j & 1, 8))) { alive = false; break; }
+      tcgen05_fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, x[g]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * g < cols) tmem_load_wait(x[g]);
+      if (negative) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[g][i] ^= 0x80000000u;
+      }
+      if (j * KEYS + cols - 1 > first) {
+        const int limit = last_key - j * KEYS;                 // columns above it are not this row's
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
+      }
+      float best = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * g < cols) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) best = fmaxf(best, __uint_as_float(x[g][i]));
+        }
+      if (j == 0) {
+        top = best;
+      } else if (__any_sync(0xffffffffu, (best - top) * c > 8.0f)) {
+        const float higher = fmaxf(top, best), factor = exp2_approx((top - higher) * c);
+        top = higher;
+        sum *= factor;
+        // S of this tile was issued after the previous tile's O += P V and has arrived: O is complete
+#pragma unroll 1
+        for (int g = 0; g < HD / 32; ++g) {
+          uint32_t o[32];
+          tmem_load_32(o_addr + 32 * g, o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+          tmem_store_32(o_addr + 32 * g, o);
+        }
+      }
+      const float shift = top * c - kLift;
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        if (32 * g < cols) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = exp2_approx(__uint_as_float(x[g][2 * i]) * c - shift);
+            const float b = exp2_approx(__uint_as_float(x[g][2 * i + 1]) * c - shift);
+            part[(2 * i) & 3] += a;
+            part[(2 * i + 1) & 3] += b;
+            packed[i] = pack2<T>(a, b);
+          }
+          tmem_store_16(s_addr + 16 * g, packed);
+        }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (j * KEYS + cols > item.length) {
+        // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
+        if (!__all_sync(0xffffffffu, wait(v_full(j % RING), (j / RING) & 1, 8))) { alive = false; break; }
+        clear_rows<BOXES>(v_ring + (j % RING) * TILE, item.length - j * KEYS, cols, thread, 128);
+      }
+      tmem_store_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(s));
+    }
+    if (alive && count && __all_sync(0xffffffffu, wait(o_full(s), 0, 8))) {
+      tcgen05_fence_after();
+      const float factor = 1.0f / sum;
+      const bool mine = token < item.length;
+      const int64_t row = (static_cast<int64_t>(item.start) + token) * p.heads + head;
+      T* dst = static_cast<T*>(p.out) + row * p.dim;
+      if (mine && p.lse) p.lse[row] = top * c + log2f(sum) - kLift;
+#pragma unroll 1
+      for (int g = 0; g < HD / 32; ++g) {
+        uint32_t o[32];
+        tmem_load_32(o_addr + 32 * g, o);
+        if (mine) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 v;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * factor, __uint_as_float(o[8 * i + 2 * e + 1]) * factor);
+            if (32 * g + 8 * i < p.dim) *reinterpret_cast<uint4*>(dst + 32 * g + 8 * i) = v;
+          }
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  settle(abort_flag);
+  if (warp == 9) tmem_free(tmem);
+}
+
+// ---- backward ------------------------------------------------------------------------
+// Two kernels that each recompute the probabilities, instead of one that would have to add query gradients from many key
+// tiles into memory: 14 instead of 10 FLOP per pair and channel, but no atomics and no order that changes the sums.
+//
+// fp16 keeps 10 more bits of range for small probabilities: P is formed as 2^10 P (at most 1024) and the factor is
+// taken out of dv at the end and out of dS where it is formed.
+template <typename T> struct Lift {
+  static constexpr float kBits = std::is_same<T, __half>::value ? 10.0f : 0.0f;
+  static constexpr float kInverse = std::is_same<T, __half>::value ? 0x1p-10f : 1.0f;
+};
+constexpr int kBackwardThreads = 384;      // two elementwise warpgroups and one that holds the copy, MMA and statistics warps
+
+// A operand in TMEM: k step k (16 columns of the tile) of the packed pairs; each warpgroup packs its own 64 columns over
+// the first half of where they were.
+__device__ __forceinline__ uint32_t packed_column(int k) { return (k / 4) * 64 + (k % 4) * 8; }
+
+// D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major)
+template <typename T, int HD>
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int steps, bool accumulate) {
+  const uint32_t idesc = operand_desc<T>(true, HD);
+  for (int k = 0; k < steps; ++k)
+    mma_ts(d, a + packed_column(k), desc_low(b + k * 2048, BOX_BYTES), desc_high(1024), idesc, accumulate || k > 0);
+}
+
+// dk and dv of one 128-key tile over a run of query tiles. Everything is transposed - a thread owns a KEY -, so that P^T
+// and dS^T come out of TMEM in the layout in which they go back as A operands:
+//   S^T = K Q^T, dP^T = V dY^T, dV += P^T dY, dK += dS^T Q
+// The tensor core runs dV(i), S(i + 1), dK(i), dP(i + 1): the exponentials of tile i + 1 run under dK(i) and dP(i + 1),
+// dS under dV and S. TMEM: S^T / P^T at 0, dP^T / dS^T at 128, dV at 256, dK at 384.
+template <int HD> struct KeyShape {
+  static constexpr uint32_t kTile = HD / 64 * BOX_BYTES;
+  static constexpr int kRing = 2;
+  static constexpr uint32_t kStats = 2 * 128 * 4;
+  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + kRing * kStats + 1024 + 256;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc_kernel(const __grid_constant__ AttentionParams p) {
+  using Shape = KeyShape<HD>;
+  constexpr int BOXES = HD / 64, RING = Shape::kRing;
+  constexpr uint32_t TILE = Shape::kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + TILE, q_ring = v_tile + TILE, g_ring = q_ring + RING * TILE;
+  float* stats = reinterpret_cast<float*>(smem + (2 + 2 * RING) * TILE);      // per ring stage: lse[128], delta[128]
+  const uint32_t bars = g_ring + RING * TILE + RING * Shape::kStats;
+  const uint32_t kv_full = bars, s_full = bars + 8, dp_full = bars + 16, p_ready = bars + 24, ds_ready = bars + 32, done = bars + 40;
+  auto q_full = [&](int r) { return bars + 48u + 8u * r; };
+  auto q_empty = [&](int r) { return bars + 48u + 8u * (RING + r); };
+  auto g_full = [&](int r) { return bars + 48u + 8u * (2 * RING + r); };
+  auto g_empty = [&](int r) { return bars + 48u + 8u * (3 * RING + r); };
+  auto stat_full = [&](int r) { return bars + 48u + 8u * (4 * RING + r); };
+  auto stat_empty = [&](int r) { return bars + 48u + 8u * (5 * RING + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + RING * Shape::kStats + 48 + 48 * RING);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    for (int r = 0; r < RING; ++r) {
+      mbar_init(q_full(r), 1);
+      mbar_init(q_empty(r), 1);
+      mbar_init(g_full(r), 1);
+      mbar_init(g_empty(r), 1);
+      mbar_init(stat_full(r), 1);
+      mbar_init(stat_empty(r), 8);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(tmem_slot));
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Waiter wait{abort_flag, p.error_flag};
+
+  const PlanRecord item = p.items[2 * (blockIdx.x / p.kv_heads)], range = p.items[2 * (blockIdx.x / p.kv_heads) + 1];
+  const int shared = blockIdx.x % p.kv_heads, key0 = item.a, slot = item.b;
+  const int first = range.start, count = range.length - range.start;          // query tiles of this piece
+  const int per_block = (item.length - key0 + p.tile_tokens - 1) / p.tile_tokens;
+  const int group0 = shared * (p.heads / p.kv_heads);
+  // query tile i of the piece: its first token in the document and first head
+  auto tile_token = [&](int i) { return key0 + ((first + i) % per_block) * p.tile_tokens; };
+  auto tile_head = [&](int i) { return group0 + ((first + i) / per_block) * p.packed; };
+
+  if (warp >= 8) {
+    registers_down<104>();
+    if (warp == 8) {
+      if (lane == 0) {
+        mbar_expect_tx(kv_full, 2 * TILE);
+        for (int b = 0; b < BOXES; ++b) tma_load_3d(k_tile + b * BOX_BYTES, &p.k, kv_full, 64 * b, shared, item.start + key0);
+        for (int b = 0; b < BOXES; ++b) tma_load_3d(v_tile + b * BOX_BYTES, &p.v, kv_full, 64 * b, shared, item.start + key0);
+        for (int i = 0; i < count; ++i) {
+          const int r = i % RING;
+          const uint32_t free_parity = ((i / RING) & 1) ^ 1;
+          const int token = item.start + tile_token(i), head = tile_head(i);
+          if (!wait(q_empty(r), free_parity, 6)) break;
+          mbar_expect_tx(q_full(r), TILE);
+          for (int b = 0; b < BOXES; ++b) tma_load_3d(q_ring + r * TILE + b * BOX_BYTES, &p.q, q_full(r), 64 * b, head, token);
+          if (!wait(g_empty(r), free_parity, 6)) break;
+          mbar_expect_tx(g_full(r), TILE);
+          for (int b = 0; b < BOXES; ++b) tma_load_3d(g_ring + r * TILE + b * BOX_BYTES, &p.dy, g_full(r), 64 * b, head, token);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      if (lane == 0) {
+        bool alive = wait(kv_full, 0, 7) && wait(q_full(0), 0, 7);
+        if (alive) {
+          tcgen05_fence_after();
+          product_nt<T, HD>(tmem, k_tile, q_ring, 128);
+          umma_commit(s_full);
+          alive = wait(g_full(0), 0, 7);
+          if (alive) {
+            product_nt<T, HD>(tmem + 128, v_tile, g_ring, 128);
+            umma_commit(dp_full);
+          }
+        }
+        for (int i = 0; i < count && alive; ++i) {
+          const int r = i % RING, next = (i + 1) % RING;
+          const uint32_t next_parity = ((i + 1) / RING) & 1;
+          if (!wait(p_ready, i & 1, 7)) break;
+          tcgen05_fence_after();
+          product_tn<T, HD>(tmem + 256, tmem, g_ring + r * TILE, 8, i > 0);
+          umma_commit(g_empty(r));
+          if (i + 1 < count) {
+            if (!wait(q_full(next), next_parity, 7)) break;
+            product_nt<T, HD>(tmem, k_tile, q_ring + next * TILE, 128);
+            umma_commit(s_full);
+          }
+          if (!wait(ds_ready, i & 1, 7)) break;
+          tcgen05_fence_after();
+          product_tn<T, HD>(tmem + 384, tmem + 128, q_ring + r * TILE, 8, i > 0);
+          umma_commit(q_empty(r));
+          if (i + 1 < count) {
+            if (!wait(g_full(next), next_parity, 7)) break;
+            product_nt<T, HD>(tmem + 128, v_tile, g_ring + next * TILE, 128);
+            umma_commit(dp_full);
+          } else {
+            umma_commit(done);
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 10) {
+      for (int i = 0; i < count; ++i) {
+        const int r = i % RING;
+        const int token0 = tile_token(i), head0 = tile_head(i);
+        float values[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = lane + 32 * e, token = token0 + row / p.packed;
+          const int64_t at = (static_cast<int64_t>(item.start) + token) * p.heads + head0 + row % p.packed;
+          const bool inside = token < item.length;
+          values[0][e] = inside ? p.lse[at] - Lift<T>::kBits : 0.0f;
+          values[1][e] = inside ? p.delta[at] * Lift<T>::kInverse : 0.0f;
+        }
+        if (!__all_sync(0xffffffffu, wait(stat_empty(r), ((i / RING) & 1) ^ 1, 6))) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          stats[r * 256 + lane + 32 * e] = values[0][e];
+          stats[r * 256 + 128 + lane + 32 * e] = values[1][e];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(stat_full(r));
+      }
+    }
+  } else {
+    registers_up<200>();
+    const int half = warp >> 2, thread = threadIdx.x & 127;
+    const int key = key0 + thread;
+    const float c = p.scale * kLog2e;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    const uint32_t s_addr = tmem + lanes + 64 * half, dp_addr = s_addr + 128;
+    bool alive = true;
+    for (int i = 0; i < count; ++i) {
+      const int r = i % RING;
+      const int token0 = tile_token(i);
+      // this thread's columns [low, high) of the tile: queries at or after its key, inside the document
+      const bool partial = token0 < key0 + 127 || token0 + p.tile_tokens > item.length;
+      const int low = (key - token0) * p.packed - 64 * half, high = (item.length - token0) * p.packed - 64 * half;
+      const float4* lse4 = reinterpret_cast<const float4*>(stats + r * 256 + 64 * half);
+      const float4* delta4 = lse4 + 32;
+      if (!__all_sync(0xffffffffu, wait(stat_full(r), (i / RING) & 1, 8) && wait(s_full, i & 1, 8))) { alive = false; break; }
+      tcgen05_fence_after();
+      float prob[64];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+      for (int g = 0; g < 2; ++g) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float4 l = lse4[e];
+        prob[4 * e] = exp2_approx(prob[4 * e] * c - l.x);
+        prob[4 * e + 1] = exp2_approx(prob[4 * e + 1] * c - l.y);
+        prob[4 * e + 2] = exp2_approx(prob[4 * e + 2] * c - l.z);
+        prob[4 * e + 3] = exp2_approx(prob[4 * e + 3] * c - l.w);
+      }
+      if (partial) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < low || e >= high) prob[e] = 0.0f;
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(prob[32 * g + 2 * e], prob[32 * g + 2 * e + 1]);
+        tmem_store_16(s_addr + 16 * g, packed);
+      }
+      if (token0 + p.tile_tokens > item.length) {
+        // rows of dY and Q behind the document's end must not meet the zeros of P and dS
+        if (!__all_sync(0xffffffffu, wait(g_full(r), (i / RING) & 1, 8))) { alive = false; break; }
+        const int from = (item.length - token0) * p.packed;
+        clear_rows<BOXES>(g_ring + r * TILE, from, 128, threadIdx.x, 256);
+        clear_rows<BOXES>(q_ring + r * TILE, from, 128, threadIdx.x, 256);
+      }
+      tmem_store_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      if (!__all_sync(0xffffffffu, wait(dp_full, i & 1, 8))) { alive = false; break; }
+      tcgen05_fence_after();
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t x[32], packed[16];
+        tmem_load_32(dp_addr + 32 * g, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float4 d = delta4[8 * g + e];
+          const float delta[4] = {d.x, d.y, d.z, d.w};
+          float slope[4];
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const int at = 4 * e + f;
+            slope[f] = prob[32 * g + at] * (__uint_as_float(x[at]) * Lift<T>::kInverse - delta[f]);
+          }
+          if (partial) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              const int at = 32 * g + 4 * e + f;
+              if (at < low || at >= high) slope[f] = 0.0f;
+            }
+          }
+          packed[2 * e] = pack2<T>(slope[0], slope[1]);
+          packed[2 * e + 1] = pack2<T>(slope[2], slope[3]);
+        }
+        // chunk g goes over columns that chunk 0 has been read from
+        tmem_store_16(dp_addr + 16 * g, packed);
+      }
+      tmem_store_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(stat_empty(r));
+        mbar_arrive(ds_ready);
+      }
+    }
+    if (alive && __all_sync(0xffffffffu, wait(done, 0, 8))) {
+      tcgen05_fence_after();
+      const bool mine = key < item.length;
+      const int64_t row = (static_cast<int64_t>(item.start) + key) * p.kv_heads + shared;
+#pragma unroll 1
+      for (int g = 0; g < HD / 32; ++g) {
+        // half 0 takes dk, half 1 dv
+        uint32_t o[32];
+        tmem_load_32(tmem + lanes + (half ? 256 : 384) + 32 * g, o);
+        const float factor = half ? Lift<T>::kInverse : p.scale;
+        if (mine && slot < 0) {
+          T* dst = static_cast<T*>(half ? p.dv : p.dk) + row * p.dim + 32 * g;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 v;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              w[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]) * factor, __uint_as_float(o[8 * e + 2 * f + 1]) * factor);
+            if (32 * g + 8 * e < p.dim) *reinterpret_cast<uint4*>(dst + 8 * e) = v;
+          }
+        } else if (mine) {
+          float* dst = p.partials + (((static_cast<int64_t>(slot) * p.kv_heads + shared) * 2 + half) * 128 + thread) * p.dim + 32 * g;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (32 * g + 4 * e < p.dim)
+              *reinterpret_cast<float4*>(dst + 4 * e) =
+                  make_float4(__uint_as_float(o[4 * e]) * factor, __uint_as_float(o[4 * e + 1]) * factor,
+                              __uint_as_float(o[4 * e + 2]) * factor, __uint_as_float(o[4 * e + 3]) * factor);
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  settle(abort_flag);
+  if (warp == 9) tmem_free(tmem);
+}
+
+// dk (z = 0) and dv (z = 1) of the key tiles that were cut into pieces: the pieces' shares added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_sum_pieces_kernel(const __grid_constant__ AttentionParams p) {
+  const PlanRecord r = p.items[blockIdx.x];            // (first token, rows, first slot, slots)
+  const int shared = blockIdx.y, which = blockIdx.z, quads = p.dim / 4;
+  T* out = static_cast<T*>(which ? p.dv : p.dk);
+  const int64_t step = static_cast<int64_t>(p.kv_heads) * 2 * 128 * p.dim;
+  const float* base = p.partials + ((static_cast<int64_t>(r.a) * p.kv_heads + shared) * 2 + which) * 128 * p.dim;
+  for (int i = threadIdx.x; i < r.length * quads; i += 256) {
+    const float* src = base + 4 * i;
+    float4 sum = *reinterpret_cast<const float4*>(src);
+    for (int s = 1; s < r.b; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(src + s * step);
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    const int row = i / quads, at = 4 * (i % quads);
+    *reinterpret_cast<uint2*>(out + ((static_cast<int64_t>(r.start) + row) * p.kv_heads + shared) * p.dim + at) =
+        make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
+  }
+}
+
+// dq of one 128-row tile over the document's keys: S = Q K^T, dP = dY V^T, dQ += dS K. A thread owns a row (two
+// threads share it, 64 columns each). S has two buffers and dS goes back over its own S, so dP(j + 1) may start as soon
+// as dP(j) has been read: the tensor core runs dP(j + 1), dQ(j), S(j + 2) under the exponentials of tile j + 1.
+// TMEM: S at 0 and 128, dP at 256, dQ at 384.
+template <int HD> struct QueryShape {
+  static constexpr uint32_t kTile = HD / 64 * BOX_BYTES;
+  static constexpr int kKeyRing = 3, kValueRing = 2;
+  static constexpr size_t kSmem = (2 + kKeyRing + kValueRing) * kTile + 1024 + 256;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_tc_kernel(const __grid_constant__ AttentionParams p) {
+  using Shape = QueryShape<HD>;
+  constexpr int BOXES = HD / 64, KR = Shape::kKeyRing, VR = Shape::kValueRing;
+  constexpr uint32_t TILE = Shape::kTile;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t q_tile = smem_u32(smem), g_tile = q_tile + TILE, k_ring = g_tile + TILE, v_ring = k_ring + KR * TILE;
+  const uint32_t bars = v_ring + VR * TILE;
+  const uint32_t q_full = bars, g_full = bars + 8, dp_full = bars + 16, ds_ready = bars + 24, done = bars + 32;
+  auto s_full = [&](int b) { return bars + 40u + 8u * b; };
+  auto k_full = [&](int r) { return bars + 56u + 8u * r; };
+  auto k_empty = [&](int r) { return bars + 56u + 8u * (KR + r); };
+  auto v_full = [&](int r) { return bars + 56u + 8u * (2 * KR + r); };
+  auto v_empty = [&](int r) { return bars + 56u + 8u * (2 * KR + VR + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + KR + VR) * TILE + 56 + 16 * (KR + VR));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(g_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(done, 1);
+    for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1);
+    for (int r = 0; r < KR; ++r) {
+      mbar_init(k_full(r), 1);
+      mbar_init(k_empty(r), 1);
+    }
+    for (int r = 0; r < VR; ++r) {
+      mbar_init(v_full(r), 1);
+      mbar_init(v_empty(r), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(tmem_slot));
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Waiter wait{abort_flag, p.error_flag};
+
+  const PlanRecord item = p.items[blockIdx.x / p.head_blocks];
+  const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
+  const int shared = head0 / (p.heads / p.kv_heads);
+  const int end = min(item.length, item.a + p.tile_tokens);        // keys [0, end) are all this tile can see
+  const int n = (end + KEYS - 1) / KEYS;
+  auto columns = [&](int j) { return min(KEYS, (end - j * KEYS + 31) & ~31); };
+
+  if (warp >= 8) {
+    registers_down<104>();
+    if (warp == 8) {
+      if (lane == 0) {
+        const int token = item.start + item.a;
+        mbar_expect_tx(q_full, TILE);
+        for (int b = 0; b < BOXES; ++b) tma_load_3d(q_tile + b * BOX_BYTES, &p.q, q_full, 64 * b, head0, token);
+        for (int j = 0; j < n; ++j) {
+          const int kr = j % KR, vr = j % VR;
+          if (!wait(k_empty(kr), ((j / KR) & 1) ^ 1, 6)) break;
+          mbar_expect_tx(k_full(kr), TILE);
+          for (int b = 0; b < BOXES; ++b) tma_load_3d(k_ring + kr * TILE + b * BOX_BYTES, &p.k, k_full(kr), 64 * b, shared, item.start + j * KEYS);
+          if (j == 0) {
+            mbar_expect_tx(g_full, TILE);
+            for (int b = 0; b < BOXES; ++b) tma_load_3d(g_tile + b * BOX_BYTES, &p.dy, g_full, 64 * b, head0, token);
+          }
+          if (!wait(v_empty(vr), ((j / VR) & 1) ^ 1, 6)) break;
+          mbar_expect_tx(v_full(vr), TILE);
+          for (int b = 0; b < BOXES; ++b) tma_load_3d(v_ring + vr * TILE + b * BOX_BYTES, &p.v, v_full(vr), 64 * b, shared, item.start + j * KEYS);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      if (lane == 0) {
+        auto scores = [&](int j) {
+          product_nt<T, HD>(tmem + (j & 1) * 128, q_tile, k_ring + (j % KR) * TILE, columns(j));
+          umma_commit(s_full(j & 1));
+        };
+        auto slopes = [&](int j) {
+          product_nt<T, HD>(tmem + 256, g_tile, v_ring + (j % VR) * TILE, columns(j));
+          umma_commit(dp_full);
+          umma_commit(v_empty(j % VR));
+        };
+        bool alive = wait(q_full, 0, 7) && wait(k_full(0), 0, 7);
+        if (alive) {
+          tcgen05_fence_after();
+          scores(0);
+          alive = wait(g_full, 0, 7) && wait(v_full(0), 0, 7);
+          if (alive) slopes(0);
+        }
+        if (alive && n > 1) {
+          alive = wait(k_full(1), 0, 7);
+          if (alive) scores(1);
+        }
+        for (int j = 0; j < n && alive; ++j) {
+          if (!wait(ds_ready, j & 1, 7)) break;
+          tcgen05_fence_after();
+          if (j + 1 < n) {
+            if (!wait(v_full((j + 1) % VR), ((j + 1) / VR) & 1, 7)) break;
+            slopes(j + 1);
+          }
+          product_tn<T, HD>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, columns(j) / 16, j > 0);
+          umma_commit(k_empty(j % KR));
+          if (j + 2 < n) {
+            if (!wait(k_full((j + 2) % KR), ((j + 2) / KR) & 1, 7)) break;
+            scores(j + 2);
+          }
+          if (j + 1 == n) umma_commit(done);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    registers_up<200>();
+    const int half = warp >> 2, thread = threadIdx.x & 127;
+    const int token = item.a + thread / p.packed, head = head0 + thread % p.packed;
+    const bool mine = token < item.length;
+    const int64_t row = (static_cast<int64_t>(item.start) + token) * p.heads + head;
+    const float c = p.scale * kLog2e;
+    const float lse = mine ? p.lse[row] : 0.0f, delta = mine ? p.delta[row] : 0.0f;
+    const int last_key = min(token, item.length - 1);
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
+    bool alive = true;
+    for (int j = 0; j < n; ++j) {
+      const int cols = columns(j) - 64 * half;                   // of this warpgroup's 64: the first `cols`, if any
+      const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + 64 * half, dp_addr = tmem + lanes + 256 + 64 * half;
+      const bool partial = j * KEYS + columns(j) - 1 > item.a;
+      const int limit = last_key - j * KEYS - 64 * half;         // columns above it are not this row's
+      if (!__all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, 8))) { alive = false; break; }
+      tcgen05_fence_after();
+      float prob[64];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (32 * g < cols) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (32 * g < cols) {
+#pragma unroll
+          for (int e = 32 * g; e < 32 * g + 32; ++e) prob[e] = exp2_approx(prob[e] * c - lse);
+        }
+      if (!__all_sync(0xffffffffu, wait(dp_full, j & 1, 8))) { alive = false; break; }
+      tcgen05_fence_after();
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (32 * g < cols) {
+          uint32_t x[32], packed[16];
+          tmem_load_32(dp_addr + 32 * g, x);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(prob[32 * g + e] * (__uint_as_float(x[e]) - delta));
+          if (partial) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * g + e > limit) x[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+          tmem_store_16(s_addr + 16 * g, packed);
+        }
+      if (j * KEYS + columns(j) > item.length)                   // rows of K behind the document's end
+        clear_rows<BOXES>(k_ring + (j % KR) * TILE, item.length - j * KEYS, columns(j), threadIdx.x, 256);
+      tmem_store_wait();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (alive && __all_sync(0xffffffffu, wait(done, 0, 8))) {
+      tcgen05_fence_after();
+      T* dst = static_cast<T*>(p.out) + row * p.dim + half * (HD / 2);
+#pragma unroll 1
+      for (int g = 0; g < HD / 64; ++g) {
+        uint32_t o[32];
+        tmem_load_32(tmem + lanes + 384 + half * (HD / 2) + 32 * g, o);
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint4 v;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              w[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]) * p.scale, __uint_as_float(o[8 * e + 2 * f + 1]) * p.scale);
+            if (half * (HD / 2) + 32 * g + 8 * e < p.dim) *reinterpret_cast<uint4*>(dst + 32 * g + 8 * e) = v;
+          }
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  settle(abort_flag);
+  if (warp == 9) tmem_free(tmem);
+}
+
+// ---- host side -------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 encode_function() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult status;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &status) != cudaSuccess ||
+        status != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+// Boxes of 64 channels x `box_heads` heads x `box_tokens` tokens over [tokens, heads, dim].
+int heads_map(CUtensorMap* map, const HeadsView& view, int64_t tokens, int heads, int dim, int box_heads, int box_tokens, int dtype) {
+  auto fn = encode_function();
+  if (!fn) return fail(CT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(view.head_stride) * 2, static_cast<cuuint64_t>(view.token_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult rc = fn(map, dtype == CT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(view.data), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(CT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)rc);
+  return CT_OK;
+}
+
+bool view_ok(const HeadsView& v) {
+  return (reinterpret_cast<uintptr_t>(v.data) & 15) == 0 && v.token_stride > 0 && v.head_stride > 0 && v.token_stride % 8 == 0 &&
+         v.head_stride % 8 == 0 && v.token_stride < (int64_t(1) << 38) && v.head_stride < (int64_t(1) << 38);
+}
+bool address_ok(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int fill(AttentionParams& p, const AttentionArgs& a, PlanSection which) {
+  p.items = section(a, which);
+  p.out = a.out;
+  p.lse = a.lse;
+  p.delta = a.delta;
+  p.partials = a.partials;
+  p.heads = a.heads;
+  p.kv_heads = a.kv_heads;
+  p.dim = a.head_dim;
+  p.packed = packed_heads(a.heads, a.kv_heads);
+  p.tile_tokens = 128 / p.packed;
+  p.head_blocks = a.heads / p.packed;
+  p.scale = a.scale;
+  p.error_flag = device_error_flag();
+  if (!p.error_flag) return fail(CT_ERR_CUDA, "cannot allocate the device error flag");
+  int rc = heads_map(&p.q, a.q, a.tokens, a.heads, a.head_dim, p.packed, p.tile_tokens, a.dtype);
+  if (!rc) rc = heads_map(&p.k, a.k, a.tokens, a.kv_heads, a.head_dim, 1, KEYS, a.dtype);
+  if (!rc) rc = heads_map(&p.v, a.v, a.tokens, a.kv_heads, a.head_dim, 1, KEYS, a.dtype);
+  return rc;
+}
+
+int launch_tc(const char* name, void (*kernel)(AttentionParams), const AttentionParams& p, int64_t blocks, int threads, size_t smem,
+              cudaStream_t stream) {
+  if (blocks > 0x7fffffff) return fail(CT_ERR_UNSUPPORTED, "%s: %lld blocks", name, (long long)blocks);
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (err != cudaSuccess) return fail(CT_ERR_CUDA, "%s: %s", name, cudaGetErrorString(err));
+  kernel<<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
+  count_launch(true);
+  return check_launch(name);
+}
+
+template <typename T, int HD> int forward(const AttentionArgs& a, const AttentionParams& p, cudaStream_t stream) {
+  return launch_tc("attention_forward_tc_kernel", attention_forward_tc_kernel<T, HD>, p, a.count[kPlanForward] * p.head_blocks,
+                   kForwardThreads, ForwardShape<HD>::kSmem, stream);
+}
+
+template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t stream) {
+  AttentionParams p{};
+  int rc = fill(p, a, kPlanQuery);
+  const HeadsView dy{a.dy, static_cast<int64_t>(a.heads) * a.head_dim, a.head_dim};
+  if (!rc) rc = heads_map(&p.dy, dy, a.tokens, a.heads, a.head_dim, p.packed, p.tile_tokens, a.dtype);
+  if (rc) return rc;
+  p.dk = a.dk;
+  p.dv = a.dv;
+  p.out = a.dq;
+  rc = launch_tc("attention_query_gradient_tc_kernel", attention_query_gradient_tc_kernel<T, HD>, p,
+                 a.count[kPlanQuery] * p.head_blocks, kBackwardThreads, QueryShape<HD>::kSmem, stream);
+  if (rc) return rc;
+  p.items = section(a, kPlanKeys);
+  rc = launch_tc("attention_key_gradient_tc_kernel", attention_key_gradient_tc_kernel<T, HD>, p, a.count[kPlanKeys] * p.kv_heads,
+                 kBackwardThreads, KeyShape<HD>::kSmem, stream);
+  if (rc || !a.count[kPlanReduce]) return rc;
+  p.items = section(a, kPlanReduce);
+  attention_sum_pieces_kernel<T><<<dim3(a.count[kPlanReduce], a.kv_heads, 2), 256, 0, stream>>>(p);
+  count_launch(false);
+  return check_launch("attention_sum_pieces_kernel");
+}
+
+}  // namespace
+
+bool attention_tc_supported(const AttentionArgs& a) {
+  return (a.dtype == CT_BF16 || a.dtype == CT_F16) && a.head_dim % 8 == 0 && a.head_dim <= 128 && view_ok(a.q) && view_ok(a.k) &&
+         view_ok(a.v) && address_ok(a.out) && address_ok(a.dy) && address_ok(a.dq) && address_ok(a.dk) && address_ok(a.dv);
+}
+
+int attention_tc_forward(const AttentionArgs& a, cudaStream_t stream) {
+  AttentionParams p{};
+  const int rc = fill(p, a, kPlanForward);
+  if (rc) return rc;
+  if (a.dtype == CT_BF16) return a.head_dim <= 64 ? forward<__nv_bfloat16, 64>(a, p, stream) : forward<__nv_bfloat16, 128>(a, p, stream);
+  return a.head_dim <= 64 ? forward<__half, 64>(a, p, stream) : forward<__half, 128>(a, p, stream);
+}
+
+int64_t attention_tc_workspace(int64_t key_slots, int kv_heads, int head_dim) { return key_slots * kv_heads * head_dim * 128 * 8; }
+
+int attention_tc_backward(const AttentionArgs& a, cudaStream_t stream) {
+  if (a.dtype == CT_BF16) return a.head_dim <= 64 ? backward<__nv_bfloat16, 64>(a, stream) : backward<__nv_bfloat16, 128>(a, stream);
+  return a.head_dim <= 64 ? backward<__half, 64>(a, stream) : backward<__half, 128>(a, stream);
+}
+
 }  // namespace ct

@@ -8,6 +8,10 @@ Bounds, for a type with rounding error u (half a step, torch.finfo(t).eps / 2) a
                 the product with v, 0 where it stays in 32 bits
   delta         sum |dy| (dy_bound + head_dim e |y|)          (it is formed from the rounded y)
   dS            (w + r)|dS| + P (head_dim e |dy|.|v| + delta's bound)
+                in fp16 values below 2^-14 have an absolute step: 2^-25 for dS, 2^-35 and 2^-32 for the probabilities of dv
+                and of the output, which are kept 2^10 and 2^7 above their size
+                the 16-bit path's exponential flushes results below 2^-126 to zero: an absolute step of 2^-126 per
+                probability, times what it multiplies
   dv, dq, dk    the same sums over absolute values, times 1 + (terms) e, plus u of the result
 """
 
@@ -18,7 +22,8 @@ def reference(q, k, v, spans, scale, dy=None, rounded=True):
     """(values, bounds): dicts of y and, with dy, dq, dk, dv. Tokens of no document: zero, and a bound of zero."""
     u = torch.finfo(q.dtype).eps / 2
     w = u if rounded else 0.0
-    e = 2.0 ** -24
+    t = 2.0 ** -25 if rounded and q.dtype == torch.float16 else 0.0
+    e, f = 2.0 ** -24, 2.0 ** -126
     dim, group = q.shape[-1], q.shape[2] // k.shape[2]
     names = ("y",) if dy is None else ("y", "dq", "dk", "dv")
     like = {"y": q, "dq": q, "dk": k, "dv": v}
@@ -37,7 +42,7 @@ def reference(q, k, v, spans, scale, dy=None, rounded=True):
             ds = (dim + 4) * e * abs(scale) * (qd.abs() @ kd.abs().T)
             r = 2 * float(ds.max()) + n * e + 2.0 ** -20
             y = p @ vd
-            spread = (w + r) * (p @ vd.abs())
+            spread = (w + r) * (p @ vd.abs()) + (t * 2 ** -7 + f) * (allowed.double() @ vd.abs())
             y_error = spread + u * (y.abs() + spread)
             values["y"][row, start:end, h], errors["y"][row, start:end, h] = y, y_error
             if dy is None:
@@ -47,9 +52,10 @@ def reference(q, k, v, spans, scale, dy=None, rounded=True):
             dp, delta = g @ vd.T, (g * y).sum(-1, keepdim=True)
             delta_error = (g.abs() * (y_error + dim * e * y.abs())).sum(-1, keepdim=True)
             slope = p * (dp - delta)
-            slope_error = (w + r) * slope.abs() + p * (dim * e * (g.abs() @ vd.abs().T) + delta_error)
+            seen = allowed.double()
+            slope_error = (w + r) * slope.abs() + (t + f * (dp - delta).abs()) * seen + p * (dim * e * (g.abs() @ vd.abs().T) + delta_error)
             values["dv"][row, start:end, s] += p.T @ g
-            errors["dv"][row, start:end, s] += ((w + r) * p.T @ g.abs()) * terms + (n * group) * e * (p.T @ g.abs())
+            errors["dv"][row, start:end, s] += (((w + r) * p + (t * 2 ** -10 + f) * seen).T @ g.abs()) * terms + (n * group) * e * (p.T @ g.abs())
             values["dq"][row, start:end, h] = slope @ kd * scale
             errors["dq"][row, start:end, h] = abs(scale) * ((slope_error * terms + n * e * slope.abs()) @ kd.abs())
             values["dk"][row, start:end, s] += slope.T @ qd * scale
