@@ -40,6 +40,36 @@ __device__ __forceinline__ float exp2_approx(float x) {   // special-function un
   return y;
 }
 
+// Two fp32 lanes per instruction: halves the issue slots of everything between the exponentials.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Keeps the code behind a rare condition behind a branch (the compiler would rather compute it always and select).
+__device__ __forceinline__ void rare() { asm volatile("" ::: "memory"); }
+
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -67,15 +97,44 @@ template <typename T> __device__ __forceinline__ uint32_t operand_desc(bool b_mn
   return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t chosen;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+  return chosen != 0;
+}
+// A value that all lanes hold, in a form that the compiler knows to be uniform.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ PlanRecord uniform(PlanRecord r) { return {uniform(r.start), uniform(r.length), uniform(r.a), uniform(r.b)}; }
+
+// The MMA warp walks its loops as a whole - with uniform control flow descriptors stay in uniform registers, and a chain
+// of MMAs costs few instructions each - and one elected lane issues. (With one lane in the loop an MMA took 110 cycles to issue.)
 // scores: D[128, n] = A[128, HD] . B[n, HD]^T, both tiles as 128-row boxes of 64 channels
 template <typename T, int HD>
 __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, int n) {
-  const uint32_t idesc = operand_desc<T>(false, n);
+  const uint32_t idesc = operand_desc<T>(false, n), a_lo = desc_low(a, 16), b_lo = desc_low(b, 16);
+  if (elect_one()) {
 #pragma unroll
-  for (int k = 0; k < HD / 16; ++k) {
-    const uint32_t offset = (k / 4) * BOX_BYTES + (k % 4) * 32;
-    mma_ss(d, desc_low(a + offset, 16), desc_low(b + offset, 16), desc_high(1024), idesc, k > 0);
+    for (int k = 0; k < HD / 16; ++k) {
+      const uint32_t offset = ((k / 4) * BOX_BYTES + (k % 4) * 32) >> 4;
+      mma_ss(d, a_lo + offset, b_lo + offset, desc_high(1024), idesc, k > 0);
+    }
   }
+}
+
+// D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major). K step k (16 rows of B) of A starts at
+// column k / SPAN * STRIDE + k % SPAN * 8.
+template <typename T, int HD, int SPAN, int STRIDE>
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int steps, bool accumulate) {
+  const uint32_t idesc = operand_desc<T>(true, HD), b_lo = desc_low(b, BOX_BYTES);
+  if (elect_one()) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < steps)
+        mma_ts(d, a + k / SPAN * STRIDE + k % SPAN * 8, b_lo + k * (2048 >> 4), desc_high(1024), idesc, accumulate || k > 0);
+  }
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (elect_one()) umma_commit(bar);
 }
 
 __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t* r) {
@@ -128,12 +187,30 @@ struct AttentionParams {
   int* error_flag;
 };
 
-// The waiting side of the barriers of one CTA (bounded, see tcgen05.cuh).
+// The waiting side of the barriers of one CTA. Bounded like mbar_wait (tcgen05.cuh), but the clock is read only after
+// some tries: reading it costs a few hundred cycles, during which the tensor core runs dry.
 struct Waiter {
   volatile int* abort_flag;
   int* error_flag;
   __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, int code) const {
-    return mbar_wait_until(bar, parity, abort_flag, error_flag, code, kWaitLimitNs);
+    uint64_t start = 0;
+    for (uint32_t tries = 1; !mbar_try_wait(bar, parity); ++tries) {
+      if ((tries & 63u) == 0) {
+        if (*abort_flag) return false;
+        const uint64_t now = global_timer_ns();
+        if (start == 0) start = now;
+        if (now - start > kWaitLimitNs) {
+          *abort_flag = 1;
+          atomicCAS(error_flag, 0, code);
+          return false;
+        }
+      }
+    }
+    return true;
+  }
+  // by a whole warp, which stays together
+  __device__ __forceinline__ bool warp(uint32_t bar, uint32_t parity, int code) const {
+    return __all_sync(0xffffffffu, (*this)(bar, parity, code));
   }
 };
 
@@ -185,7 +262,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 64 + 32 * RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(q_full(s), 1);
@@ -207,10 +284,10 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const Waiter wait{abort_flag, p.error_flag};
 
-  const PlanRecord item = p.items[blockIdx.x / p.head_blocks];
+  const PlanRecord item = uniform(p.items[blockIdx.x / p.head_blocks]);
   const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
   const int shared = head0 / (p.heads / p.kv_heads);
   // stage s holds the tokens from item.a + s * tile_tokens; keys [0, end[s]) are all it can see
@@ -254,42 +331,36 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     }
     __syncwarp();
    } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t value_desc = desc_high(1024);
-      auto scores = [&](int s, int j) {
-        product_nt<T, HD>(tmem + s * 128, q_tile + s * TILE, k_ring + (j % RING) * TILE, columns(s ? end1 : end0, j));
-        umma_commit(s_full(s));
-      };
-      bool alive = wait(q_full(0), 0, 7) && wait(k_full(0), 0, 7);
-      if (alive) {
-        tcgen05_fence_after();
-        scores(0, 0);
-        if (n1) {
-          alive = wait(q_full(1), 0, 7);
-          if (alive) scores(1, 0);
-        }
-        umma_commit(k_empty(0));
+    auto scores = [&](int s, int j) {
+      product_nt<T, HD>(tmem + s * 128, q_tile + s * TILE, k_ring + (j % RING) * TILE, columns(s ? end1 : end0, j));
+      commit(s_full(s));
+    };
+    bool alive = wait.warp(q_full(0), 0, 7) && wait.warp(k_full(0), 0, 7);
+    if (alive) {
+      tcgen05_fence_after();
+      scores(0, 0);
+      if (n1) {
+        alive = wait.warp(q_full(1), 0, 7);
+        if (alive) scores(1, 0);
       }
-      for (int j = 0; j < n && alive; ++j) {
-        const int r = j % RING, next = (j + 1) % RING;
-        if (!wait(v_full(r), (j / RING) & 1, 7)) break;
-        for (int s = 0; s < 2; ++s) {
-          const int count = s ? n1 : n0, end = s ? end1 : end0;
-          if (j < count) {
-            if (!wait(p_full(s), j & 1, 7)) { alive = false; break; }
-            tcgen05_fence_after();
-            const uint32_t idesc = operand_desc<T>(true, HD);
-            const int steps = columns(end, j) / 16;
-            for (int k = 0; k < steps; ++k)
-              mma_ts(tmem + kOutColumn + s * 128, tmem + s * 128 + 8 * k, desc_low(v_ring + r * TILE + k * 2048, BOX_BYTES), value_desc,
-                     idesc, j > 0 || k > 0);
-            if (j + 1 == count) umma_commit(o_full(s));
-          }
-          if (s == 1) umma_commit(v_empty(r));
-          if (j + 1 < n && s == 0 && !wait(k_full(next), ((j + 1) / RING) & 1, 7)) { alive = false; break; }
-          if (j + 1 < count) scores(s, j + 1);
-          if (s == 1 && j + 1 < n) umma_commit(k_empty(next));
+      commit(k_empty(0));
+    }
+    for (int j = 0; j < n && alive; ++j) {
+      const int r = j % RING, next = (j + 1) % RING;
+      if (!wait.warp(v_full(r), (j / RING) & 1, 7)) break;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int count = s ? n1 : n0, end = s ? end1 : end0;
+        if (j < count) {
+          if (!wait.warp(p_full(s), j & 1, 7)) { alive = false; break; }
+          tcgen05_fence_after();
+          product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, columns(end, j) / 16, j > 0);
+          if (j + 1 == count) commit(o_full(s));
         }
+        if (s == 1) commit(v_empty(r));
+        if (j + 1 < n && s == 0 && !wait.warp(k_full(next), ((j + 1) / RING) & 1, 7)) { alive = false; break; }
+        if (j + 1 < count) scores(s, j + 1);
+        if (s == 1 && j + 1 < n) commit(k_empty(next));
       }
     }
     __syncwarp();
@@ -312,7 +383,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     bool alive = true;
     for (int j = 0; j < count; ++j) {
       const int cols = columns(end, j);
-      if (!__all_sync(0xffffffffu, wait(s_full(s), j & 1, 8))) { alive = false; break; }
+      if (!wait.warp(s_full(s), j & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
       uint32_t x[4][32];
 #pragma unroll
@@ -322,12 +393,14 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
       for (int g = 0; g < 4; ++g)
         if (32 * g < cols) tmem_load_wait(x[g]);
       if (negative) {
+        rare();
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[g][i] ^= 0x80000000u;
       }
       if (j * KEYS + cols - 1 > first) {
+        rare();
         const int limit = last_key - j * KEYS;                 // columns above it are not this row's
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -335,13 +408,15 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
           for (int i = 0; i < 32; ++i)
             if (32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
       }
-      float best = -INFINITY;
+      float peak[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // four chains of three-way maxima
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (32 * g < cols) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) best = fmaxf(best, __uint_as_float(x[g][i]));
+          for (int i = 0; i < 16; ++i)
+            peak[i & 3] = max3(peak[i & 3], __uint_as_float(x[g][2 * i]), __uint_as_float(x[g][2 * i + 1]));
         }
+      const float best = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
       if (j == 0) {
         top = best;
       } else if (__any_sync(0xffffffffu, (best - top) * c > 8.0f)) {
@@ -359,25 +434,27 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
         }
       }
       const float shift = top * c - kLift;
-      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float2 c2 = make_float2(c, c), shift2 = make_float2(-shift, -shift);
+      float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         if (32 * g < cols) {
           uint32_t packed[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = exp2_approx(__uint_as_float(x[g][2 * i]) * c - shift);
-            const float b = exp2_approx(__uint_as_float(x[g][2 * i + 1]) * c - shift);
-            part[(2 * i) & 3] += a;
-            part[(2 * i + 1) & 3] += b;
-            packed[i] = pack2<T>(a, b);
+            float2 e = fma2(make_float2(__uint_as_float(x[g][2 * i]), __uint_as_float(x[g][2 * i + 1])), c2, shift2);
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
+            part[i & 1] = add2(part[i & 1], e);
+            packed[i] = pack2<T>(e.x, e.y);
           }
           tmem_store_16(s_addr + 16 * g, packed);
         }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      part[0] = add2(part[0], part[1]);
+      sum += part[0].x + part[0].y;
       if (j * KEYS + cols > item.length) {
         // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
-        if (!__all_sync(0xffffffffu, wait(v_full(j % RING), (j / RING) & 1, 8))) { alive = false; break; }
+        if (!wait.warp(v_full(j % RING), (j / RING) & 1, 8)) { alive = false; break; }
         clear_rows<BOXES>(v_ring + (j % RING) * TILE, item.length - j * KEYS, cols, thread, 128);
       }
       tmem_store_wait();
@@ -385,7 +462,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full(s));
     }
-    if (alive && count && __all_sync(0xffffffffu, wait(o_full(s), 0, 8))) {
+    if (alive && count && wait.warp(o_full(s), 0, 8)) {
       tcgen05_fence_after();
       const float factor = 1.0f / sum;
       const bool mine = token < item.length;
@@ -429,17 +506,8 @@ template <typename T> struct Lift {
 };
 constexpr int kBackwardThreads = 384;      // two elementwise warpgroups and one that holds the copy, MMA and statistics warps
 
-// A operand in TMEM: k step k (16 columns of the tile) of the packed pairs; each warpgroup packs its own 64 columns over
-// the first half of where they were.
-__device__ __forceinline__ uint32_t packed_column(int k) { return (k / 4) * 64 + (k % 4) * 8; }
-
-// D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major)
-template <typename T, int HD>
-__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int steps, bool accumulate) {
-  const uint32_t idesc = operand_desc<T>(true, HD);
-  for (int k = 0; k < steps; ++k)
-    mma_ts(d, a + packed_column(k), desc_low(b + k * 2048, BOX_BYTES), desc_high(1024), idesc, accumulate || k > 0);
-}
+// dP^T / dS and P: each warpgroup packs its own 64 columns over the first half of where they were.
+constexpr int kHalfSpan = 4, kHalfStride = 64;
 
 // dk and dv of one 128-key tile over a run of query tiles. Everything is transposed - a thread owns a KEY -, so that P^T
 // and dS^T come out of TMEM in the layout in which they go back as A operands:
@@ -473,7 +541,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + RING * Shape::kStats + 48 + 48 * RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     mbar_init(s_full, 1);
@@ -497,10 +565,11 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const Waiter wait{abort_flag, p.error_flag};
 
-  const PlanRecord item = p.items[2 * (blockIdx.x / p.kv_heads)], range = p.items[2 * (blockIdx.x / p.kv_heads) + 1];
+  const PlanRecord item = uniform(p.items[2 * (blockIdx.x / p.kv_heads)]);
+  const PlanRecord range = uniform(p.items[2 * (blockIdx.x / p.kv_heads) + 1]);
   const int shared = blockIdx.x % p.kv_heads, key0 = item.a, slot = item.b;
   const int first = range.start, count = range.length - range.start;          // query tiles of this piece
   const int per_block = (item.length - key0 + p.tile_tokens - 1) / p.tile_tokens;
@@ -530,41 +599,39 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       }
       __syncwarp();
     } else if (warp == 9) {
-      if (lane == 0) {
-        bool alive = wait(kv_full, 0, 7) && wait(q_full(0), 0, 7);
+      bool alive = wait.warp(kv_full, 0, 7) && wait.warp(q_full(0), 0, 7);
+      if (alive) {
+        tcgen05_fence_after();
+        product_nt<T, HD>(tmem, k_tile, q_ring, 128);
+        commit(s_full);
+        alive = wait.warp(g_full(0), 0, 7);
         if (alive) {
-          tcgen05_fence_after();
-          product_nt<T, HD>(tmem, k_tile, q_ring, 128);
-          umma_commit(s_full);
-          alive = wait(g_full(0), 0, 7);
-          if (alive) {
-            product_nt<T, HD>(tmem + 128, v_tile, g_ring, 128);
-            umma_commit(dp_full);
-          }
+          product_nt<T, HD>(tmem + 128, v_tile, g_ring, 128);
+          commit(dp_full);
         }
-        for (int i = 0; i < count && alive; ++i) {
-          const int r = i % RING, next = (i + 1) % RING;
-          const uint32_t next_parity = ((i + 1) / RING) & 1;
-          if (!wait(p_ready, i & 1, 7)) break;
-          tcgen05_fence_after();
-          product_tn<T, HD>(tmem + 256, tmem, g_ring + r * TILE, 8, i > 0);
-          umma_commit(g_empty(r));
-          if (i + 1 < count) {
-            if (!wait(q_full(next), next_parity, 7)) break;
-            product_nt<T, HD>(tmem, k_tile, q_ring + next * TILE, 128);
-            umma_commit(s_full);
-          }
-          if (!wait(ds_ready, i & 1, 7)) break;
-          tcgen05_fence_after();
-          product_tn<T, HD>(tmem + 384, tmem + 128, q_ring + r * TILE, 8, i > 0);
-          umma_commit(q_empty(r));
-          if (i + 1 < count) {
-            if (!wait(g_full(next), next_parity, 7)) break;
-            product_nt<T, HD>(tmem + 128, v_tile, g_ring + next * TILE, 128);
-            umma_commit(dp_full);
-          } else {
-            umma_commit(done);
-          }
+      }
+      for (int i = 0; i < count && alive; ++i) {
+        const int r = i % RING, next = (i + 1) % RING;
+        const uint32_t next_parity = ((i + 1) / RING) & 1;
+        if (!wait.warp(p_ready, i & 1, 7)) break;
+        tcgen05_fence_after();
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 256, tmem, g_ring + r * TILE, 8, i > 0);
+        commit(g_empty(r));
+        if (i + 1 < count) {
+          if (!wait.warp(q_full(next), next_parity, 7)) break;
+          product_nt<T, HD>(tmem, k_tile, q_ring + next * TILE, 128);
+          commit(s_full);
+        }
+        if (!wait.warp(ds_ready, i & 1, 7)) break;
+        tcgen05_fence_after();
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + 128, q_ring + r * TILE, 8, i > 0);
+        commit(q_empty(r));
+        if (i + 1 < count) {
+          if (!wait.warp(g_full(next), next_parity, 7)) break;
+          product_nt<T, HD>(tmem + 128, v_tile, g_ring + next * TILE, 128);
+          commit(dp_full);
+        } else {
+          commit(done);
         }
       }
       __syncwarp();
@@ -581,7 +648,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
           values[0][e] = inside ? p.lse[at] - Lift<T>::kBits : 0.0f;
           values[1][e] = inside ? p.delta[at] * Lift<T>::kInverse : 0.0f;
         }
-        if (!__all_sync(0xffffffffu, wait(stat_empty(r), ((i / RING) & 1) ^ 1, 6))) break;
+        if (!wait.warp(stat_empty(r), ((i / RING) & 1) ^ 1, 6)) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           stats[r * 256 + lane + 32 * e] = values[0][e];
@@ -607,22 +674,26 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       const int low = (key - token0) * p.packed - 64 * half, high = (item.length - token0) * p.packed - 64 * half;
       const float4* lse4 = reinterpret_cast<const float4*>(stats + r * 256 + 64 * half);
       const float4* delta4 = lse4 + 32;
-      if (!__all_sync(0xffffffffu, wait(stat_full(r), (i / RING) & 1, 8) && wait(s_full, i & 1, 8))) { alive = false; break; }
+      if (!(wait.warp(stat_full(r), (i / RING) & 1, 8) && wait.warp(s_full, i & 1, 8))) { alive = false; break; }
       tcgen05_fence_after();
       float prob[64];
 #pragma unroll
       for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
 #pragma unroll
       for (int g = 0; g < 2; ++g) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+      const float2 c2 = make_float2(c, c);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float4 l = lse4[e];
-        prob[4 * e] = exp2_approx(prob[4 * e] * c - l.x);
-        prob[4 * e + 1] = exp2_approx(prob[4 * e + 1] * c - l.y);
-        prob[4 * e + 2] = exp2_approx(prob[4 * e + 2] * c - l.z);
-        prob[4 * e + 3] = exp2_approx(prob[4 * e + 3] * c - l.w);
+        const float2 a = fma2(make_float2(prob[4 * e], prob[4 * e + 1]), c2, make_float2(-l.x, -l.y));
+        const float2 b = fma2(make_float2(prob[4 * e + 2], prob[4 * e + 3]), c2, make_float2(-l.z, -l.w));
+        prob[4 * e] = exp2_approx(a.x);
+        prob[4 * e + 1] = exp2_approx(a.y);
+        prob[4 * e + 2] = exp2_approx(b.x);
+        prob[4 * e + 3] = exp2_approx(b.y);
       }
       if (partial) {
+        rare();
 #pragma unroll
         for (int e = 0; e < 64; ++e)
           if (e < low || e >= high) prob[e] = 0.0f;
@@ -636,7 +707,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       }
       if (token0 + p.tile_tokens > item.length) {
         // rows of dY and Q behind the document's end must not meet the zeros of P and dS
-        if (!__all_sync(0xffffffffu, wait(g_full(r), (i / RING) & 1, 8))) { alive = false; break; }
+        if (!wait.warp(g_full(r), (i / RING) & 1, 8)) { alive = false; break; }
         const int from = (item.length - token0) * p.packed;
         clear_rows<BOXES>(g_ring + r * TILE, from, 128, threadIdx.x, 256);
         clear_rows<BOXES>(q_ring + r * TILE, from, 128, threadIdx.x, 256);
@@ -645,32 +716,34 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready);
-      if (!__all_sync(0xffffffffu, wait(dp_full, i & 1, 8))) { alive = false; break; }
+      if (!wait.warp(dp_full, i & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         uint32_t x[32], packed[16];
         tmem_load_32(dp_addr + 32 * g, x);
+        const float2 inverse = make_float2(Lift<T>::kInverse, Lift<T>::kInverse);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float4 d = delta4[8 * g + e];
-          const float delta[4] = {d.x, d.y, d.z, d.w};
-          float slope[4];
 #pragma unroll
-          for (int f = 0; f < 4; ++f) {
-            const int at = 4 * e + f;
-            slope[f] = prob[32 * g + at] * (__uint_as_float(x[at]) * Lift<T>::kInverse - delta[f]);
+          for (int f = 0; f < 2; ++f) {
+            const int at = 4 * e + 2 * f;
+            const float2 slope = mul2(make_float2(prob[32 * g + at], prob[32 * g + at + 1]),
+                                      fma2(make_float2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), inverse,
+                                           f ? make_float2(-d.z, -d.w) : make_float2(-d.x, -d.y)));
+            x[at] = __float_as_uint(slope.x);
+            x[at + 1] = __float_as_uint(slope.y);
           }
-          if (partial) {
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              const int at = 32 * g + 4 * e + f;
-              if (at < low || at >= high) slope[f] = 0.0f;
-            }
-          }
-          packed[2 * e] = pack2<T>(slope[0], slope[1]);
-          packed[2 * e + 1] = pack2<T>(slope[2], slope[3]);
         }
+        if (partial) {
+          rare();
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (32 * g + e < low || 32 * g + e >= high) x[e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
         // chunk g goes over columns that chunk 0 has been read from
         tmem_store_16(dp_addr + 16 * g, packed);
       }
@@ -682,7 +755,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
         mbar_arrive(ds_ready);
       }
     }
-    if (alive && __all_sync(0xffffffffu, wait(done, 0, 8))) {
+    if (alive && wait.warp(done, 0, 8)) {
       tcgen05_fence_after();
       const bool mine = key < item.length;
       const int64_t row = (static_cast<int64_t>(item.start) + key) * p.kv_heads + shared;
@@ -771,7 +844,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + KR + VR) * TILE + 56 + 16 * (KR + VR));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(g_full, 1);
@@ -795,10 +868,10 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const Waiter wait{abort_flag, p.error_flag};
 
-  const PlanRecord item = p.items[blockIdx.x / p.head_blocks];
+  const PlanRecord item = uniform(p.items[blockIdx.x / p.head_blocks]);
   const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
   const int shared = head0 / (p.heads / p.kv_heads);
   const int end = min(item.length, item.a + p.tile_tokens);        // keys [0, end) are all this tile can see
@@ -828,42 +901,40 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       }
       __syncwarp();
     } else if (warp == 9) {
-      if (lane == 0) {
-        auto scores = [&](int j) {
-          product_nt<T, HD>(tmem + (j & 1) * 128, q_tile, k_ring + (j % KR) * TILE, columns(j));
-          umma_commit(s_full(j & 1));
-        };
-        auto slopes = [&](int j) {
-          product_nt<T, HD>(tmem + 256, g_tile, v_ring + (j % VR) * TILE, columns(j));
-          umma_commit(dp_full);
-          umma_commit(v_empty(j % VR));
-        };
-        bool alive = wait(q_full, 0, 7) && wait(k_full(0), 0, 7);
-        if (alive) {
-          tcgen05_fence_after();
-          scores(0);
-          alive = wait(g_full, 0, 7) && wait(v_full(0), 0, 7);
-          if (alive) slopes(0);
+      auto scores = [&](int j) {
+        product_nt<T, HD>(tmem + (j & 1) * 128, q_tile, k_ring + (j % KR) * TILE, columns(j));
+        commit(s_full(j & 1));
+      };
+      auto slopes = [&](int j) {
+        product_nt<T, HD>(tmem + 256, g_tile, v_ring + (j % VR) * TILE, columns(j));
+        commit(dp_full);
+        commit(v_empty(j % VR));
+      };
+      bool alive = wait.warp(q_full, 0, 7) && wait.warp(k_full(0), 0, 7);
+      if (alive) {
+        tcgen05_fence_after();
+        scores(0);
+        alive = wait.warp(g_full, 0, 7) && wait.warp(v_full(0), 0, 7);
+        if (alive) slopes(0);
+      }
+      if (alive && n > 1) {
+        alive = wait.warp(k_full(1), 0, 7);
+        if (alive) scores(1);
+      }
+      for (int j = 0; j < n && alive; ++j) {
+        if (!wait.warp(ds_ready, j & 1, 7)) break;
+        tcgen05_fence_after();
+        if (j + 1 < n) {
+          if (!wait.warp(v_full((j + 1) % VR), ((j + 1) / VR) & 1, 7)) break;
+          slopes(j + 1);
         }
-        if (alive && n > 1) {
-          alive = wait(k_full(1), 0, 7);
-          if (alive) scores(1);
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, columns(j) / 16, j > 0);
+        commit(k_empty(j % KR));
+        if (j + 2 < n) {
+          if (!wait.warp(k_full((j + 2) % KR), ((j + 2) / KR) & 1, 7)) break;
+          scores(j + 2);
         }
-        for (int j = 0; j < n && alive; ++j) {
-          if (!wait(ds_ready, j & 1, 7)) break;
-          tcgen05_fence_after();
-          if (j + 1 < n) {
-            if (!wait(v_full((j + 1) % VR), ((j + 1) / VR) & 1, 7)) break;
-            slopes(j + 1);
-          }
-          product_tn<T, HD>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, columns(j) / 16, j > 0);
-          umma_commit(k_empty(j % KR));
-          if (j + 2 < n) {
-            if (!wait(k_full((j + 2) % KR), ((j + 2) / KR) & 1, 7)) break;
-            scores(j + 2);
-          }
-          if (j + 1 == n) umma_commit(done);
-        }
+        if (j + 1 == n) commit(done);
       }
       __syncwarp();
     }
@@ -883,7 +954,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + 64 * half, dp_addr = tmem + lanes + 256 + 64 * half;
       const bool partial = j * KEYS + columns(j) - 1 > item.a;
       const int limit = last_key - j * KEYS - 64 * half;         // columns above it are not this row's
-      if (!__all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, 8))) { alive = false; break; }
+      if (!wait.warp(s_full(j & 1), (j >> 1) & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
       float prob[64];
 #pragma unroll
@@ -896,9 +967,13 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       for (int g = 0; g < 2; ++g)
         if (32 * g < cols) {
 #pragma unroll
-          for (int e = 32 * g; e < 32 * g + 32; ++e) prob[e] = exp2_approx(prob[e] * c - lse);
+          for (int e = 32 * g; e < 32 * g + 32; e += 2) {
+            const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
+            prob[e] = exp2_approx(a.x);
+            prob[e + 1] = exp2_approx(a.y);
+          }
         }
-      if (!__all_sync(0xffffffffu, wait(dp_full, j & 1, 8))) { alive = false; break; }
+      if (!wait.warp(dp_full, j & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
 #pragma unroll
       for (int g = 0; g < 2; ++g)
@@ -906,8 +981,14 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
           uint32_t x[32], packed[16];
           tmem_load_32(dp_addr + 32 * g, x);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(prob[32 * g + e] * (__uint_as_float(x[e]) - delta));
+          for (int e = 0; e < 32; e += 2) {
+            const float2 slope = mul2(make_float2(prob[32 * g + e], prob[32 * g + e + 1]),
+                                      add2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(-delta, -delta)));
+            x[e] = __float_as_uint(slope.x);
+            x[e + 1] = __float_as_uint(slope.y);
+          }
           if (partial) {
+            rare();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
               if (32 * g + e > limit) x[e] = 0u;
@@ -923,7 +1004,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
     }
-    if (alive && __all_sync(0xffffffffu, wait(done, 0, 8))) {
+    if (alive && wait.warp(done, 0, 8)) {
       tcgen05_fence_after();
       T* dst = static_cast<T*>(p.out) + row * p.dim + half * (HD / 2);
 #pragma unroll 1
