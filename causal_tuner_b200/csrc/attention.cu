@@ -446,7 +446,7 @@ int describe(AttentionArgs& a, const char* name, const int32_t* plan, const int6
 int check_path(const AttentionArgs& a, const char* name, int path) {
   if (path != CT_PATH_SIMT && path != CT_PATH_TCGEN05) return fail(CT_ERR_ARG, "%s: path %d", name, path);
   if (path == CT_PATH_TCGEN05 && !attention_tc_supported(a))
-    return fail(CT_ERR_UNSUPPORTED, "%s: the tensor-core path needs 16-bit types, 16-byte aligned rows and head_dim a multiple of 8", name);
+    return fail(CT_ERR_UNSUPPORTED, "%s: the tensor-core path needs 16-bit types, 16-byte aligned rows, head_dim a multiple of 8 and a scale that is not tiny", name);
   return CT_OK;
 }
 
@@ -486,7 +486,7 @@ extern "C" int ct_attention_forward(const void* q, int64_t q_token, int64_t q_he
 }
 
 extern "C" int ct_attention_path(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
-                                 const void* v, int64_t v_token, int64_t v_head, int heads, int kv_heads, int head_dim, int dtype) {
+                                 const void* v, int64_t v_token, int64_t v_head, int heads, int kv_heads, int head_dim, float scale, int dtype) {
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || !known(dtype)) return fail(CT_ERR_ARG, "ct_attention_path: sizes");
   AttentionArgs a{};
   a.q = {q, q_token, q_head};
@@ -495,6 +495,7 @@ extern "C" int ct_attention_path(const void* q, int64_t q_token, int64_t q_head,
   a.heads = heads;
   a.kv_heads = kv_heads;
   a.head_dim = head_dim;
+  a.scale = scale;
   a.dtype = dtype;
   return attention_tc_supported(a) ? CT_PATH_TCGEN05 : CT_PATH_SIMT;
 }

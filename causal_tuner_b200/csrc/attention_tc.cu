@@ -14,6 +14,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <cmath>
+
 #include "attention.cuh"
 #include "tcgen05.cuh"
 
@@ -61,6 +63,36 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+// 2^x for x <= 128 on the FMA units, so that the special-function units (16 results per SM and cycle, which is what the
+// tensor core's pace asks of them in full) can be relieved of a share. Range reduction by rounding to the nearest integer
+// n (Cody and Waite), |x - n| <= 1/2, and a degree-5 polynomial fitted here for the smallest relative error of 2^f on
+// [-1/2, 1/2] (7.5e-8; 2.1e-7 in fp32 arithmetic, the accuracy of ex2.approx). Below 2^-125 the result stays 2^-125.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -125.0f);
+  x.y = fmaxf(x.y, -125.0f);
+  const float round = 12582912.0f;                  // 1.5 * 2^23: the sum's low mantissa bits are n
+  const float2 t = add2(x, make_float2(round, round));
+  const float2 f = add2(x, fma2(t, make_float2(-1.0f, -1.0f), make_float2(round, round)));
+  float2 r = fma2(f, make_float2(1.3276472454890609e-3f, 1.3276472454890609e-3f), make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
+  r = fma2(r, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+  r = fma2(r, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+  r = fma2(r, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+  r = fma2(r, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  r.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
+  r.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
+  return r;
+}
+// Of every 8 pairs of scores a thread turns `SHARE` on the FMA units.
+template <int SHARE> __device__ __forceinline__ constexpr bool kOnFma(int pair) { return pair % 8 < SHARE; }
+#ifndef FWD_SHARE
+#define FWD_SHARE 2
+#define KEY_SHARE 0
+#define QRY_SHARE 0
+#endif
+constexpr int kForwardShare = FWD_SHARE, kKeyShare = KEY_SHARE, kQueryShare = QRY_SHARE;
+__device__ __forceinline__ float2 exp2_pair(float2 x, bool on_fma) {
+  return on_fma ? exp2_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -122,14 +154,14 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, i
 }
 
 // D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major). K step k (16 rows of B) of A starts at
-// column k / SPAN * STRIDE + k % SPAN * 8.
+// column k / SPAN * STRIDE + k % SPAN * 8; steps [first, last).
 template <typename T, int HD, int SPAN, int STRIDE>
-__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int steps, bool accumulate) {
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int first, int last, bool accumulate) {
   const uint32_t idesc = operand_desc<T>(true, HD), b_lo = desc_low(b, BOX_BYTES);
   if (elect_one()) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (k < steps)
+      if (k >= first && k < last)
         mma_ts(d, a + k / SPAN * STRIDE + k % SPAN * 8, b_lo + k * (2048 >> 4), desc_high(1024), idesc, accumulate || k > 0);
   }
 }
@@ -253,13 +285,14 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
   const uint32_t bars = v_ring + RING * TILE;
   auto q_full = [&](int s) { return bars + 8u * s; };
   auto s_full = [&](int s) { return bars + 16u + 8u * s; };
-  auto p_full = [&](int s) { return bars + 32u + 8u * s; };
-  auto o_full = [&](int s) { return bars + 48u + 8u * s; };
-  auto k_full = [&](int r) { return bars + 64u + 8u * r; };
-  auto k_empty = [&](int r) { return bars + 64u + 8u * (RING + r); };
-  auto v_full = [&](int r) { return bars + 64u + 8u * (2 * RING + r); };
-  auto v_empty = [&](int r) { return bars + 64u + 8u * (3 * RING + r); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 64 + 32 * RING);
+  auto p_full = [&](int s, int h) { return bars + 32u + 16u * s + 8u * h; };
+  auto half_done = [&](int s) { return bars + 64u + 8u * s; };
+  auto o_full = [&](int s) { return bars + 80u + 8u * s; };
+  auto k_full = [&](int r) { return bars + 96u + 8u * r; };
+  auto k_empty = [&](int r) { return bars + 96u + 8u * (RING + r); };
+  auto v_full = [&](int r) { return bars + 96u + 8u * (2 * RING + r); };
+  auto v_empty = [&](int r) { return bars + 96u + 8u * (3 * RING + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 96 + 32 * RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -267,7 +300,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     for (int s = 0; s < 2; ++s) {
       mbar_init(q_full(s), 1);
       mbar_init(s_full(s), 1);
-      mbar_init(p_full(s), 4);
+      for (int h = 0; h < 2; ++h) mbar_init(p_full(s, h), 4);
+      mbar_init(half_done(s), 1);
       mbar_init(o_full(s), 1);
     }
     for (int r = 0; r < RING; ++r) {
@@ -352,9 +386,16 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
       for (int s = 0; s < 2; ++s) {
         const int count = s ? n1 : n0, end = s ? end1 : end0;
         if (j < count) {
-          if (!wait.warp(p_full(s), j & 1, 7)) { alive = false; break; }
+          const int steps = columns(end, j) / 16;
+          if (!wait.warp(p_full(s, 0), j & 1, 7)) { alive = false; break; }
           tcgen05_fence_after();
-          product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, columns(end, j) / 16, j > 0);
+          product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, 0, min(steps, 4), j > 0);
+          commit(half_done(s));
+          if (steps > 4) {
+            if (!wait.warp(p_full(s, 1), j & 1, 7)) { alive = false; break; }
+            tcgen05_fence_after();
+            product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, 4, steps, true);
+          }
           if (j + 1 == count) commit(o_full(s));
         }
         if (s == 1) commit(v_empty(r));
@@ -381,86 +422,94 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
     float top = -INFINITY, sum = 0.0f;
     bool alive = true;
-    for (int j = 0; j < count; ++j) {
+    const float2 c2 = make_float2(c, c);
+    for (int j = 0; j < count && alive; ++j) {
       const int cols = columns(end, j);
+      const bool partial = j * KEYS + cols - 1 > first;
+      const int limit = last_key - j * KEYS;                   // columns above it are not this row's
       if (!wait.warp(s_full(s), j & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, x[g]);
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * g < cols) tmem_load_wait(x[g]);
-      if (negative) {
-        rare();
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) x[g][i] ^= 0x80000000u;
-      }
-      if (j * KEYS + cols - 1 > first) {
-        rare();
-        const int limit = last_key - j * KEYS;                 // columns above it are not this row's
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
-      }
-      float peak[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // four chains of three-way maxima
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * g < cols) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            peak[i & 3] = max3(peak[i & 3], __uint_as_float(x[g][2 * i]), __uint_as_float(x[g][2 * i + 1]));
-        }
-      const float best = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
-      if (j == 0) {
-        top = best;
-      } else if (__any_sync(0xffffffffu, (best - top) * c > 8.0f)) {
-        const float higher = fmaxf(top, best), factor = exp2_approx((top - higher) * c);
-        top = higher;
-        sum *= factor;
-        // S of this tile was issued after the previous tile's O += P V and has arrived: O is complete
-#pragma unroll 1
-        for (int g = 0; g < HD / 32; ++g) {
-          uint32_t o[32];
-          tmem_load_32(o_addr + 32 * g, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-          tmem_store_32(o_addr + 32 * g, o);
-        }
-      }
-      const float shift = top * c - kLift;
-      const float2 c2 = make_float2(c, c), shift2 = make_float2(-shift, -shift);
-      float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (32 * g < cols) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(__uint_as_float(x[g][2 * i]), __uint_as_float(x[g][2 * i + 1])), c2, shift2);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
-            part[i & 1] = add2(part[i & 1], e);
-            packed[i] = pack2<T>(e.x, e.y);
-          }
-          tmem_store_16(s_addr + 16 * g, packed);
-        }
-      part[0] = add2(part[0], part[1]);
-      sum += part[0].x + part[0].y;
       if (j * KEYS + cols > item.length) {
         // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
         if (!wait.warp(v_full(j % RING), (j / RING) & 1, 8)) { alive = false; break; }
         clear_rows<BOXES>(v_ring + (j % RING) * TILE, item.length - j * KEYS, cols, thread, 128);
       }
-      tmem_store_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(s));
+      // Halves of 64 keys: the first half of P V runs under the exponentials of the second. The exponentials do not wait
+      // for the half's maximum: they use the maximum so far, and the half is done again with the new one in the rare
+      // case that a score is more than 2^8 above it.
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (64 * h >= cols) break;
+        uint32_t x[2][32];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 64 * h + 32 * g, x[g]);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) tmem_load_wait(x[g]);
+        if (negative) {
+          rare();
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[g][i] ^= 0x80000000u;
+        }
+        if (partial) {
+          rare();
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (64 * h + 32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
+        }
+        if (j == 0 && h == 0) {                                // key 0 is every row's: a score, not -infinity
+          rare();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top = max3(top, __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+        }
+        uint32_t packed[32];
+        float2 part[2];
+        while (true) {
+          const float shift = kLift - top * c;
+          const float2 shift2 = make_float2(shift, shift);
+          float peak[4] = {top, top, top, top};
+          part[0] = part[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float2 raw = make_float2(__uint_as_float(x[i / 16][2 * (i % 16)]), __uint_as_float(x[i / 16][2 * (i % 16) + 1]));
+            peak[i & 3] = max3(peak[i & 3], raw.x, raw.y);
+            const float2 e = exp2_pair(fma2(raw, c2, shift2), kOnFma<kForwardShare>(i));
+            part[i & 1] = add2(part[i & 1], e);
+            packed[i] = pack2<T>(e.x, e.y);
+          }
+          const float best = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
+          if (!__any_sync(0xffffffffu, (best - top) * c > 8.0f)) break;
+          rare();
+          // O holds the products of all halves so far; the last one issued has to be complete
+          const bool issued = h == 1 || j > 0;
+          if (h == 1 && !wait.warp(half_done(s), j & 1, 8)) { alive = false; break; }
+          tcgen05_fence_after();
+          const float factor = exp2_approx((top - best) * c);
+          top = best;
+          sum *= factor;
+          if (issued) {
+#pragma unroll 1
+            for (int g = 0; g < HD / 32; ++g) {
+              uint32_t o[32];
+              tmem_load_32(o_addr + 32 * g, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+              tmem_store_32(o_addr + 32 * g, o);
+            }
+          }
+        }
+        if (!alive) break;
+        part[0] = add2(part[0], part[1]);
+        sum += part[0].x + part[0].y;
+        tmem_store_32(s_addr + 32 * h, packed);
+        tmem_store_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(s, h));
+      }
     }
     if (alive && count && wait.warp(o_full(s), 0, 8)) {
       tcgen05_fence_after();
@@ -517,9 +566,39 @@ constexpr int kHalfSpan = 4, kHalfStride = 64;
 template <int HD> struct KeyShape {
   static constexpr uint32_t kTile = HD / 64 * BOX_BYTES;
   static constexpr int kRing = 2;
-  static constexpr uint32_t kStats = 2 * 128 * 4;
-  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + kRing * kStats + 1024 + 256;
+  static constexpr uint32_t kStatTile = 128 * 32;                // 128 rows x 16 values
+  static constexpr uint32_t kStats = 2 * kStatTile;              // log-sums, deltas
+  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + kStatTile + kRing * kStats + 1024 + 256;
 };
+
+// The statistics of a query tile vary along the COLUMNS of the transposed score tile, so every thread would need all of
+// them - 128 broadcast loads from shared memory per thread and tile, on the bandwidth the MMAs' operands need (1.3 of
+// 3.6 thousand cycles per tile). Instead they are subtracted by the tensor core as one more k step of 16: rows of
+// weights (the same for every key) times the value of each query split into parts of the operand type,
+//   value = 8 * w0 * part0 + w1 * part1 + w2 * part2    (k = 0..7: part0, 8: part1, 9: part2, others 0)
+// exact to 2^-24 for bf16, and for fp16 from 2^-29 up to 2^34.
+template <typename T> struct Split {
+  static constexpr float kWeight0 = std::is_same<T, __half>::value ? 32768.0f : 1.0f;
+  static constexpr float kWeight1 = std::is_same<T, __half>::value ? 256.0f : 1.0f;
+  static constexpr float kWeight2 = std::is_same<T, __half>::value ? 0.0625f : 1.0f;
+};
+// Row `row` of such a tile: K-major without swizzle, 8 x 16-byte blocks, the two k halves 2 KB apart.
+__device__ __forceinline__ void store_stat_row(uint32_t tile, int row, uint32_t eight, uint32_t two) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + row * 16), "r"(eight) : "memory");
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %2, %2};" ::"r"(tile + 2048 + row * 16), "r"(two), "r"(0) : "memory");
+}
+template <typename T> __device__ __forceinline__ void store_split(uint32_t tile, int row, float value) {
+  const float part0 = round_to<T>(value * (0.125f / Split<T>::kWeight0));
+  const float rest0 = value - part0 * (8.0f * Split<T>::kWeight0);
+  const float part1 = round_to<T>(rest0 * (1.0f / Split<T>::kWeight1));
+  const float rest1 = rest0 - part1 * Split<T>::kWeight1;
+  store_stat_row(tile, row, pack2<T>(part0, part0), pack2<T>(part1, rest1 * (1.0f / Split<T>::kWeight2)));
+}
+template <typename T> __device__ __forceinline__ void subtract_stats(uint32_t d, uint32_t weights, uint32_t stats) {
+  const uint32_t plain = desc_high(128) & ~(7u << 29);           // no swizzle, 8-row groups 128 bytes apart
+  const uint32_t idesc = operand_desc<T>(false, 128), a_lo = desc_low(weights, 2048), b_lo = desc_low(stats, 2048);
+  if (elect_one()) umma_bf16(d, a_lo, plain, b_lo, plain, idesc, 1);
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc_kernel(const __grid_constant__ AttentionParams p) {
@@ -529,8 +608,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t k_tile = smem_u32(smem), v_tile = k_tile + TILE, q_ring = v_tile + TILE, g_ring = q_ring + RING * TILE;
-  float* stats = reinterpret_cast<float*>(smem + (2 + 2 * RING) * TILE);      // per ring stage: lse[128], delta[128]
-  const uint32_t bars = g_ring + RING * TILE + RING * Shape::kStats;
+  const uint32_t weights = g_ring + RING * TILE, stats = weights + Shape::kStatTile;      // per ring stage: log-sums, deltas
+  const uint32_t bars = stats + RING * Shape::kStats;
   const uint32_t kv_full = bars, s_full = bars + 8, dp_full = bars + 16, p_ready = bars + 24, ds_ready = bars + 32, done = bars + 40;
   auto q_full = [&](int r) { return bars + 48u + 8u * r; };
   auto q_empty = [&](int r) { return bars + 48u + 8u * (RING + r); };
@@ -538,7 +617,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
   auto g_empty = [&](int r) { return bars + 48u + 8u * (3 * RING + r); };
   auto stat_full = [&](int r) { return bars + 48u + 8u * (4 * RING + r); };
   auto stat_empty = [&](int r) { return bars + 48u + 8u * (5 * RING + r); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + RING * Shape::kStats + 48 + 48 * RING);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + Shape::kStatTile + RING * Shape::kStats + 48 + 48 * RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -555,10 +634,14 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       mbar_init(g_full(r), 1);
       mbar_init(g_empty(r), 1);
       mbar_init(stat_full(r), 1);
-      mbar_init(stat_empty(r), 8);
+      mbar_init(stat_empty(r), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_shared();
+  }
+  if (threadIdx.x < 128) {
+    store_stat_row(weights, threadIdx.x, pack2<T>(Split<T>::kWeight0, Split<T>::kWeight0), pack2<T>(Split<T>::kWeight1, Split<T>::kWeight2));
     fence_async_shared();
   }
   if (warp == 9) tmem_alloc(smem_u32(tmem_slot));
@@ -599,43 +682,49 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       }
       __syncwarp();
     } else if (warp == 9) {
-      bool alive = wait.warp(kv_full, 0, 7) && wait.warp(q_full(0), 0, 7);
+      auto scores = [&](int r) {                                 // log2 P / c
+        product_nt<T, HD>(tmem, k_tile, q_ring + r * TILE, 128);
+        subtract_stats<T>(tmem, weights, stats + r * Shape::kStats);
+        commit(s_full);
+      };
+      auto slopes = [&](int r) {                                 // dP - delta
+        product_nt<T, HD>(tmem + 128, v_tile, g_ring + r * TILE, 128);
+        subtract_stats<T>(tmem + 128, weights, stats + r * Shape::kStats + Shape::kStatTile);
+        commit(dp_full);
+        commit(stat_empty(r));
+      };
+      bool alive = wait.warp(kv_full, 0, 7) && wait.warp(q_full(0), 0, 7) && wait.warp(stat_full(0), 0, 7);
       if (alive) {
         tcgen05_fence_after();
-        product_nt<T, HD>(tmem, k_tile, q_ring, 128);
-        commit(s_full);
+        scores(0);
         alive = wait.warp(g_full(0), 0, 7);
-        if (alive) {
-          product_nt<T, HD>(tmem + 128, v_tile, g_ring, 128);
-          commit(dp_full);
-        }
+        if (alive) slopes(0);
       }
       for (int i = 0; i < count && alive; ++i) {
         const int r = i % RING, next = (i + 1) % RING;
         const uint32_t next_parity = ((i + 1) / RING) & 1;
         if (!wait.warp(p_ready, i & 1, 7)) break;
         tcgen05_fence_after();
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 256, tmem, g_ring + r * TILE, 8, i > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 256, tmem, g_ring + r * TILE, 0, 8, i > 0);
         commit(g_empty(r));
         if (i + 1 < count) {
-          if (!wait.warp(q_full(next), next_parity, 7)) break;
-          product_nt<T, HD>(tmem, k_tile, q_ring + next * TILE, 128);
-          commit(s_full);
+          if (!wait.warp(q_full(next), next_parity, 7) || !wait.warp(stat_full(next), next_parity, 7)) break;
+          scores(next);
         }
         if (!wait.warp(ds_ready, i & 1, 7)) break;
         tcgen05_fence_after();
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + 128, q_ring + r * TILE, 8, i > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + 128, q_ring + r * TILE, 0, 8, i > 0);
         commit(q_empty(r));
         if (i + 1 < count) {
           if (!wait.warp(g_full(next), next_parity, 7)) break;
-          product_nt<T, HD>(tmem + 128, v_tile, g_ring + next * TILE, 128);
-          commit(dp_full);
+          slopes(next);
         } else {
           commit(done);
         }
       }
       __syncwarp();
     } else if (warp == 10) {
+      const float per_score = -1.0f / (p.scale * kLog2e);
       for (int i = 0; i < count; ++i) {
         const int r = i % RING;
         const int token0 = tile_token(i), head0 = tile_head(i);
@@ -645,15 +734,16 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
           const int row = lane + 32 * e, token = token0 + row / p.packed;
           const int64_t at = (static_cast<int64_t>(item.start) + token) * p.heads + head0 + row % p.packed;
           const bool inside = token < item.length;
-          values[0][e] = inside ? p.lse[at] - Lift<T>::kBits : 0.0f;
-          values[1][e] = inside ? p.delta[at] * Lift<T>::kInverse : 0.0f;
+          values[0][e] = inside ? (p.lse[at] - Lift<T>::kBits) * per_score : 0.0f;
+          values[1][e] = inside ? -p.delta[at] : 0.0f;
         }
         if (!wait.warp(stat_empty(r), ((i / RING) & 1) ^ 1, 6)) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          stats[r * 256 + lane + 32 * e] = values[0][e];
-          stats[r * 256 + 128 + lane + 32 * e] = values[1][e];
+          store_split<T>(stats + r * Shape::kStats, lane + 32 * e, values[0][e]);
+          store_split<T>(stats + r * Shape::kStats + Shape::kStatTile, lane + 32 * e, values[1][e]);
         }
+        fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(stat_full(r));
       }
@@ -672,25 +762,18 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       // this thread's columns [low, high) of the tile: queries at or after its key, inside the document
       const bool partial = token0 < key0 + 127 || token0 + p.tile_tokens > item.length;
       const int low = (key - token0) * p.packed - 64 * half, high = (item.length - token0) * p.packed - 64 * half;
-      const float4* lse4 = reinterpret_cast<const float4*>(stats + r * 256 + 64 * half);
-      const float4* delta4 = lse4 + 32;
-      if (!(wait.warp(stat_full(r), (i / RING) & 1, 8) && wait.warp(s_full, i & 1, 8))) { alive = false; break; }
+      if (!wait.warp(s_full, i & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
       float prob[64];
 #pragma unroll
       for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
 #pragma unroll
       for (int g = 0; g < 2; ++g) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
-      const float2 c2 = make_float2(c, c);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float4 l = lse4[e];
-        const float2 a = fma2(make_float2(prob[4 * e], prob[4 * e + 1]), c2, make_float2(-l.x, -l.y));
-        const float2 b = fma2(make_float2(prob[4 * e + 2], prob[4 * e + 3]), c2, make_float2(-l.z, -l.w));
-        prob[4 * e] = exp2_approx(a.x);
-        prob[4 * e + 1] = exp2_approx(a.y);
-        prob[4 * e + 2] = exp2_approx(b.x);
-        prob[4 * e + 3] = exp2_approx(b.y);
+      for (int e = 0; e < 64; e += 2) {
+        const float2 a = exp2_pair(mul2(make_float2(prob[e], prob[e + 1]), make_float2(c, c)), kOnFma<kKeyShare>(e / 2));
+        prob[e] = a.x;
+        prob[e + 1] = a.y;
       }
       if (partial) {
         rare();
@@ -722,19 +805,12 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       for (int g = 0; g < 2; ++g) {
         uint32_t x[32], packed[16];
         tmem_load_32(dp_addr + 32 * g, x);
-        const float2 inverse = make_float2(Lift<T>::kInverse, Lift<T>::kInverse);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float4 d = delta4[8 * g + e];
-#pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const int at = 4 * e + 2 * f;
-            const float2 slope = mul2(make_float2(prob[32 * g + at], prob[32 * g + at + 1]),
-                                      fma2(make_float2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), inverse,
-                                           f ? make_float2(-d.z, -d.w) : make_float2(-d.x, -d.y)));
-            x[at] = __float_as_uint(slope.x);
-            x[at + 1] = __float_as_uint(slope.y);
-          }
+        for (int e = 0; e < 32; e += 2) {
+          float2 slope = mul2(make_float2(prob[32 * g + e], prob[32 * g + e + 1]), make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+          if constexpr (Lift<T>::kBits != 0.0f) slope = mul2(slope, make_float2(Lift<T>::kInverse, Lift<T>::kInverse));
+          x[e] = __float_as_uint(slope.x);
+          x[e + 1] = __float_as_uint(slope.y);
         }
         if (partial) {
           rare();
@@ -750,10 +826,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       tmem_store_wait();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(stat_empty(r));
-        mbar_arrive(ds_ready);
-      }
+      if (lane == 0) mbar_arrive(ds_ready);
     }
     if (alive && wait.warp(done, 0, 8)) {
       tcgen05_fence_after();
@@ -928,7 +1001,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
           if (!wait.warp(v_full((j + 1) % VR), ((j + 1) / VR) & 1, 7)) break;
           slopes(j + 1);
         }
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, columns(j) / 16, j > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, 0, columns(j) / 16, j > 0);
         commit(k_empty(j % KR));
         if (j + 2 < n) {
           if (!wait.warp(k_full((j + 2) % KR), ((j + 2) / KR) & 1, 7)) break;
@@ -968,9 +1041,10 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
         if (32 * g < cols) {
 #pragma unroll
           for (int e = 32 * g; e < 32 * g + 32; e += 2) {
-            const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
-            prob[e] = exp2_approx(a.x);
-            prob[e + 1] = exp2_approx(a.y);
+            const float2 a = exp2_pair(fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse)),
+                                       kOnFma<kQueryShare>(e / 2));
+            prob[e] = a.x;
+            prob[e + 1] = a.y;
           }
         }
       if (!wait.warp(dp_full, j & 1, 8)) { alive = false; break; }
@@ -1126,8 +1200,12 @@ template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t 
 
 }  // namespace
 
+// The backward pass divides the log-sums by the scale (Split): a scale that would take them out of range goes to the
+// shape-generic kernels.
+bool scale_ok(const AttentionArgs& a) { return std::fabs(a.scale) >= (a.dtype == CT_F16 ? 1e-6f : 1e-20f); }
+
 bool attention_tc_supported(const AttentionArgs& a) {
-  return (a.dtype == CT_BF16 || a.dtype == CT_F16) && a.head_dim % 8 == 0 && a.head_dim <= 128 && view_ok(a.q) && view_ok(a.k) &&
+  return scale_ok(a) && (a.dtype == CT_BF16 || a.dtype == CT_F16) && a.head_dim % 8 == 0 && a.head_dim <= 128 && view_ok(a.q) && view_ok(a.k) &&
          view_ok(a.v) && address_ok(a.out) && address_ok(a.dy) && address_ok(a.dq) && address_ok(a.dk) && address_ok(a.dv);
 }
 

@@ -168,17 +168,17 @@ def attention_forward(q, k, v, plan, *, scale=None, keep_lse=True):
     library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q):
-        path = _path(library, operands, heads, plan.kv_heads, dim, code)
+        path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
         _lib.check(library.ct_attention_forward(
             *operands, out.data_ptr(), _lib.pointer(lse), plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads,
             dim, scale, code, path, _lib.stream_of(q)))
     return out, lse
 
 
-def _path(library, operands, heads, kv_heads, dim, code):
+def _path(library, operands, heads, kv_heads, dim, scale, code):
     if _lib.gemm_path == _lib.PATH_SIMT:
         return _lib.PATH_SIMT
-    return library.ct_attention_path(*operands, heads, kv_heads, dim, code)
+    return library.ct_attention_path(*operands, heads, kv_heads, dim, scale, code)
 
 
 def attention_backward(dy, q, k, v, y, lse, plan, *, scale=None):
@@ -199,7 +199,7 @@ def attention_backward(dy, q, k, v, y, lse, plan, *, scale=None):
     library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q):
-        path = _path(library, operands, heads, plan.kv_heads, dim, code)
+        path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
         size = library.ct_attention_backward_workspace(tokens, heads, plan.kv_heads, dim, plan.key_slots, path)
         workspace = torch.empty(size, device=q.device, dtype=torch.uint8)
         _lib.check(library.ct_attention_backward(

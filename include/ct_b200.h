@@ -495,7 +495,7 @@ CT_API int ct_adamw_update(int count, void* const* grads, void* const* params, v
 CT_API int ct_attention_tile_tokens(int heads, int kv_heads);
 CT_API int ct_attention_path(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                              int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int heads, int kv_heads,
-                             int head_dim, int dtype);
+                             int head_dim, float scale, int dtype);
 CT_API int ct_attention_forward(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                                 int64_t k_head, const void* v, int64_t v_token, int64_t v_head, void* out, float* lse,
                                 const int32_t* plan, const int64_t* sections, int64_t tokens, int heads, int kv_heads,

@@ -111,8 +111,8 @@ def test_entry_points_check_their_arguments():
     assert forward(sections=some) == _lib.ERR_ARG and b"plan" in library.ct_last_error()
     assert forward(dim=136) == _lib.ERR_UNSUPPORTED
     assert library.ct_attention_tile_tokens(5, 2) == _lib.ERR_ARG
-    assert library.ct_attention_path(*strides, 4, 1, 64, 9) == _lib.ERR_ARG
-    assert library.ct_attention_path(*strides, 4, 1, 64, _lib.F32) == _lib.PATH_SIMT
+    assert library.ct_attention_path(*strides, 4, 1, 64, 1.0, 9) == _lib.ERR_ARG
+    assert library.ct_attention_path(*strides, 4, 1, 64, 1.0, _lib.F32) == _lib.PATH_SIMT
     # statistics, then the larger of nothing / one fp32 row per head / one 128-row share per slot
     assert library.ct_attention_backward_workspace(100, 4, 4, 64, 0, _lib.PATH_SIMT) == 1792
     assert library.ct_attention_backward_workspace(100, 4, 1, 64, 0, _lib.PATH_SIMT) == 1792 + 2 * 100 * 4 * 64 * 4
