@@ -83,14 +83,6 @@ __device__ __forceinline__ float2 exp2_fma(float2 x) {
   r.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
   return r;
 }
-// Of every 8 pairs of scores a thread turns `SHARE` on the FMA units.
-template <int SHARE> __device__ __forceinline__ constexpr bool kOnFma(int pair) { return pair % 8 < SHARE; }
-#ifndef FWD_SHARE
-#define FWD_SHARE 2
-#define KEY_SHARE 0
-#define QRY_SHARE 0
-#endif
-constexpr int kForwardShare = FWD_SHARE, kKeyShare = KEY_SHARE, kQueryShare = QRY_SHARE;
 __device__ __forceinline__ float2 exp2_pair(float2 x, bool on_fma) {
   return on_fma ? exp2_fma(x) : make_float2(exp2_approx(x.x), exp2_approx(x.y));
 }
@@ -476,7 +468,9 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
           for (int i = 0; i < 32; ++i) {
             const float2 raw = make_float2(__uint_as_float(x[i / 16][2 * (i % 16)]), __uint_as_float(x[i / 16][2 * (i % 16) + 1]));
             peak[i & 3] = max3(peak[i & 3], raw.x, raw.y);
-            const float2 e = exp2_pair(fma2(raw, c2, shift2), kOnFma<kForwardShare>(i));
+            float2 e = fma2(raw, c2, shift2);
+            e.x = exp2_approx(e.x);
+            e.y = exp2_approx(e.y);
             part[i & 1] = add2(part[i & 1], e);
             packed[i] = pack2<T>(e.x, e.y);
           }
@@ -769,9 +763,11 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
 #pragma unroll
       for (int g = 0; g < 2; ++g) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+      // a quarter on the FMA units: 944 us of 978 without at 4 x 4096 tokens, 32 heads; an eighth 956, a half 965 (the
+      // forward and the query-gradient kernel are no faster with any share)
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
-        const float2 a = exp2_pair(mul2(make_float2(prob[e], prob[e + 1]), make_float2(c, c)), kOnFma<kKeyShare>(e / 2));
+        const float2 a = exp2_pair(mul2(make_float2(prob[e], prob[e + 1]), make_float2(c, c)), e % 16 < 4);
         prob[e] = a.x;
         prob[e + 1] = a.y;
       }
@@ -1041,10 +1037,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
         if (32 * g < cols) {
 #pragma unroll
           for (int e = 32 * g; e < 32 * g + 32; e += 2) {
-            const float2 a = exp2_pair(fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse)),
-                                       kOnFma<kQueryShare>(e / 2));
-            prob[e] = a.x;
-            prob[e + 1] = a.y;
+            const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
+            prob[e] = exp2_approx(a.x);
+            prob[e + 1] = exp2_approx(a.y);
           }
         }
       if (!wait.warp(dp_full, j & 1, 8)) { alive = false; break; }
