@@ -70,6 +70,9 @@ SIGNATURES = {
     "ct_attention_backward_workspace": (_L, [_L, _I, _I, _I, _L, _I]),
     "ct_attention_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _F, _I, _I,
                                    _P, _P]),
+    "ct_embedding_forward": (_I, [_P, _P, _P, _L, _L, _L, _F, _I, _I, _P]),
+    "ct_embedding_gradient_workspace": (_L, [_L, _L, _L]),
+    "ct_embedding_gradient": (_I, [_P, _L, _P, _P, _L, _L, _L, _F, _L, _I, _I, _P, _P]),
     "ct_adamw_update": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _F, _F, _F, _F, _L, _I, _P]),
 }
 

@@ -238,8 +238,12 @@ extern "C" int ct_check_device(void* stream) {
   cudaMemset(flag, 0, sizeof(int));
   static const char* roles[] = {"", "TMA producer waiting for a free stage", "MMA issuer waiting for a free accumulator",
                                 "MMA issuer waiting for a filled stage", "epilogue waiting for a finished accumulator",
-                                "the self-test's wait on a barrier that nothing completes"};
-  return fail(CT_ERR_DEVICE, "a tcgen05 GEMM CTA gave up on a bounded wait: %s", value >= 1 && value <= 5 ? roles[value] : "?");
+                                "the self-test's wait on a barrier that nothing completes",
+                                "attention's copies or statistics waiting for a free slot",
+                                "attention's MMA issuer waiting for an operand", "attention's warpgroups waiting for a product"};
+  if (value == 9) return fail(CT_ERR_DEVICE, "a token id lies outside the embedding table");
+  return fail(CT_ERR_DEVICE, "a tcgen05 %s CTA gave up on a bounded wait: %s", value >= 6 ? "attention" : "GEMM",
+              value >= 1 && value <= 8 ? roles[value] : "?");
 }
 
 extern "C" int ct_selftest_bounded_wait(int64_t limit_us, void* stream) {

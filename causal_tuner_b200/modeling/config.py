@@ -20,6 +20,7 @@ class ModelConfig:
     pad_token_id: int = 0
     eos_token_id: int = 1
     attention_bias: bool = True
+    embed_scale: float = 1.0            # factor of the token embeddings (1 in the reference, which has no such field)
 
     def __post_init__(self):
         if self.num_key_value_heads != 1 or self.hidden_size != self.num_attention_heads * self.head_dim:

@@ -25,6 +25,8 @@ class Runtime:
     train_embed: bool = False
     train_head: bool = False
     frozen: tuple = ()
+    # "flash_attention_2": the library's kernels (the reference's setting); "documents": this package's kernels
+    # (kernels/attention_cuda.py), any document layout without gathering; "vanilla": dense fp32, small shapes only
     attention: str = "flash_attention_2"
     mlp_tile: int | None = None
     mlp_cache_budget_bytes: int | None = None
@@ -146,6 +148,7 @@ class Attention(nn.Module):
 
     def forward(self, x, cosine, sine, segments, spans, layout=None, *, residual=None):
         from ..kernels.attention import dense_attention, flash_dense
+        from ..kernels.attention_cuda import document_attention
         from ..kernels.linear import project_group
         b, s, _ = x.shape
         c, r = self.config, self.runtime
@@ -155,6 +158,8 @@ class Attention(nn.Module):
         v = v.reshape(b, s, 1, c.head_dim)
         if r.attention == "vanilla":
             y = dense_attention(q, k, v, segments)
+        elif r.attention == "documents":
+            y = document_attention(q, k, v, layout)
         else:
             y = flash_dense(q, k, v, spans, layout=layout)
         return project_group((self.o_proj,), y.reshape(b, s, -1), r.projection_tile, residual=residual)[0]
@@ -223,6 +228,8 @@ class CausalLM(nn.Module):
     def forward(self, batch):
         from torch.utils.checkpoint import checkpoint
         from ..kernels.attention import prepare_dense_layout
+        from ..kernels.attention_cuda import prepare_documents
+        from ..kernels.embedding_cuda import embed_tokens
         from ..segments import canonical_segments, position_ids, runs
         from .rotary import rotary_values
         r = self.runtime
@@ -234,8 +241,15 @@ class CausalLM(nn.Module):
             raise ValueError("position_ids exceed the model's logical position range")
         spans = batch.get("_spans") or runs(segments)
         cosine, sine = rotary_values(positions, self.config, r.compute_dtype)
-        x = self.model.embed_tokens(batch["input_ids"]).to(r.compute_dtype)
-        layout = prepare_dense_layout(x.shape[:2], spans, x.device) if r.attention == "flash_attention_2" else None
+        table = self.model.embed_tokens
+        x = embed_tokens(batch["input_ids"], table.weight, scale=self.config.embed_scale, dtype=r.compute_dtype,
+                         padding_idx=table.padding_idx)
+        layout = None
+        if r.attention == "flash_attention_2":
+            layout = prepare_dense_layout(x.shape[:2], spans, x.device)
+        elif r.attention == "documents":
+            layout = prepare_documents(x.shape[:2], spans, x.device, self.config.num_attention_heads,
+                                       self.config.num_key_value_heads)
         recompute = r.checkpoint and self.training and torch.is_grad_enabled()
         # MLP activation cache: layers keep gate/up (instead of recomputing them in backward) while
         # the byte budget lasts, last layers first (modeling/model.py:228-239 of the reference).

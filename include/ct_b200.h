@@ -40,7 +40,7 @@ enum {
   CT_ERR_ARG = -1,          /* null pointer, negative size, unknown dtype */
   CT_ERR_UNSUPPORTED = -2,  /* shape/alignment the requested path cannot take */
   CT_ERR_CUDA = -3,         /* a CUDA runtime/driver call failed */
-  CT_ERR_DEVICE = -4        /* a kernel reported a bounded-wait timeout */
+  CT_ERR_DEVICE = -4        /* a kernel reported a bounded-wait timeout or a token id outside the embedding */
 };
 
 /* GEMM path selection. AUTO picks the tcgen05 kernel when every operand meets
@@ -507,6 +507,24 @@ CT_API int ct_attention_backward(const void* q, int64_t q_token, int64_t q_head,
                                  const float* lse, const void* dy, void* dq, void* dk, void* dv, const int32_t* plan,
                                  const int64_t* sections, int64_t tokens, int heads, int kv_heads, int head_dim,
                                  float scale, int dtype, int path, void* workspace, void* stream);
+
+/* ---- token embedding ----------------------------------------------------------------
+ * Stand in for nn.Embedding and its cast in the decoder (modeling/model.py:160-165,229 of the reference), and for its
+ * backward pass when the embedding trains (modeling/model.py:185-193).
+ * ct_embedding_forward: out[t, :] = round(scale * table[ids[t], :]) in `out_dtype`; table [rows, width] contiguous.
+ * ct_embedding_gradient: d_table[i, :] = scale * sum of dy[t, :] over the tokens with ids[t] == i, in fp32 in the order of
+ *   t (runs of more than 128 tokens: pieces of the sorted order, added in order), rounded once to `table_dtype`; zero
+ *   for every other row and for row `padding` (-1: none). The whole [rows, width] matrix is written. dy has `ld` elements
+ *   between rows. No atomics: repeated calls are bit-identical.
+ *   `workspace`: ct_embedding_gradient_workspace bytes, 256-byte aligned.
+ * An id outside [0, rows) reads as a row of zeros, gets no gradient, and makes the next ct_check_device of the device
+ * return CT_ERR_DEVICE. */
+CT_API int ct_embedding_forward(const int64_t* ids, const void* table, void* out, int64_t tokens, int64_t rows,
+                                int64_t width, float scale, int table_dtype, int out_dtype, void* stream);
+CT_API int64_t ct_embedding_gradient_workspace(int64_t tokens, int64_t rows, int64_t width);
+CT_API int ct_embedding_gradient(const void* dy, int64_t ld, const int64_t* ids, void* d_table, int64_t tokens,
+                                 int64_t rows, int64_t width, float scale, int64_t padding, int dy_dtype,
+                                 int table_dtype, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

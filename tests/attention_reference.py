@@ -10,8 +10,8 @@ Bounds, for a type with rounding error u (half a step, torch.finfo(t).eps / 2) a
   dS            (w + r)|dS| + P (head_dim e |dy|.|v| + delta's bound)
                 in fp16 values below 2^-14 have an absolute step: 2^-25 for dS, 2^-35 and 2^-32 for the probabilities of dv
                 and of the output, which are kept 2^10 and 2^7 above their size
-                the 16-bit path's exponential flushes results below 2^-126 to zero: an absolute step of 2^-126 per
-                probability, times what it multiplies
+                the 16-bit path's exponentials flush results below 2^-126 to zero, or (those on the FMA units) hold them at
+                2^-125: an absolute step of 2^-125 per probability, times what it multiplies
   dv, dq, dk    the same sums over absolute values, times 1 + (terms) e, plus u of the result
 """
 
@@ -23,7 +23,7 @@ def reference(q, k, v, spans, scale, dy=None, rounded=True):
     u = torch.finfo(q.dtype).eps / 2
     w = u if rounded else 0.0
     t = 2.0 ** -25 if rounded and q.dtype == torch.float16 else 0.0
-    e, f = 2.0 ** -24, 2.0 ** -126
+    e, f = 2.0 ** -24, 2.0 ** -125
     dim, group = q.shape[-1], q.shape[2] // k.shape[2]
     names = ("y",) if dy is None else ("y", "dq", "dk", "dv")
     like = {"y": q, "dq": q, "dk": k, "dv": v}
