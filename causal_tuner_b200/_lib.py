@@ -132,7 +132,8 @@ def require_cuda(*tensors):
 
 def stream_of(tensor):
     """Raw handle of the current stream of the tensor's device."""
-    return torch.cuda.current_stream(tensor.device).cuda_stream
+    # torch.cuda.current_stream(...).cuda_stream without building a Stream object (2 us a call)
+    return torch._C._cuda_getCurrentRawStream(tensor.device.index)
 
 
 class on_device:

@@ -17,10 +17,27 @@ namespace {
 constexpr int TILE = 64, THREADS = 256, PITCH_S = TILE + 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Rows [row0, row0 + 64) of head `head` of one document into shared memory as fp32; rows at or past `length` and
+// Four neighbouring elements as fp32 (p is aligned to four elements).
+template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
+  struct alignas(4 * sizeof(T)) Four { T v[4]; };
+  const Four f = *reinterpret_cast<const Four*>(p);
+  return make_float4(to_float<T>(f.v[0]), to_float<T>(f.v[1]), to_float<T>(f.v[2]), to_float<T>(f.v[3]));
+}
+
+// Rows [row0, row0 + 64) of one head of one document into shared memory as fp32; rows at or past `length` and
 // channels at or past `dim` are zeros, whatever memory holds there.
 template <typename T, int HD>
 __device__ __forceinline__ void load_tile(float* dst, const T* base, int64_t token_stride, int row0, int length, int dim) {
+  if (dim % 4 == 0 && token_stride % 4 == 0 && reinterpret_cast<uintptr_t>(base) % (4 * sizeof(T)) == 0) {
+#pragma unroll
+    for (int i = threadIdx.x; i < TILE * HD / 4; i += THREADS) {
+      const int r = i / (HD / 4), c = 4 * (i % (HD / 4));
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row0 + r < length && c < dim) v = load4<T>(base + (row0 + r) * token_stride + c);
+      *reinterpret_cast<float4*>(dst + r * (HD + 4) + c) = v;
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < TILE * HD; i += THREADS) {
     const int r = i / HD, c = i % HD;
     float v = 0.0f;
@@ -29,7 +46,8 @@ __device__ __forceinline__ void load_tile(float* dst, const T* base, int64_t tok
   }
 }
 
-// acc[i][j] = sum over channels of a[ty + 16 i] . b[tx + 16 j]
+// A thread's 4 x 4 part of a 64 x 64 tile: rows 4 ty + i, columns tx + 16 j.
+// acc[i][j] = sum over channels of a[4 ty + i] . b[tx + 16 j]
 template <int HD>
 __device__ __forceinline__ void tile_dot(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
 #pragma unroll
@@ -40,7 +58,7 @@ __device__ __forceinline__ void tile_dot(float (&acc)[4][4], const float* a, con
   for (int c = 0; c < HD; c += 4) {
     float4 x[4], y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * (HD + 4) + c);
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * (HD + 4) + c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (HD + 4) + c);
 #pragma unroll
@@ -51,23 +69,32 @@ __device__ __forceinline__ void tile_dot(float (&acc)[4][4], const float* a, con
   }
 }
 
-// acc[i][g] += sum over n of w(ty + 16 i, n) * b[n][4 tx + 64 g ..]; w is read at w[row * PITCH_S + n], or with
+// acc[i][g] += sum over n of w(4 ty + i, n) * b[n][4 tx + 64 g ..]; w is read at w[row * PITCH_S + n], or with
 // TRANSPOSED at w[n * PITCH_S + row].
 template <int HD, bool TRANSPOSED>
 __device__ __forceinline__ void tile_product(float4 (&acc)[4][HD / 64], const float* w, const float* b, int ty, int tx) {
-#pragma unroll 4
-  for (int n = 0; n < TILE; ++n) {
-    float x[4];
+#pragma unroll 2
+  for (int n = 0; n < TILE; n += 4) {
+    float x[4][4];                                    // [n][i]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = TRANSPOSED ? w[n * PITCH_S + ty + 16 * i] : w[(ty + 16 * i) * PITCH_S + n];
-#pragma unroll
-    for (int g = 0; g < HD / 64; ++g) {
-      const float4 y = *reinterpret_cast<const float4*>(b + n * (HD + 4) + 4 * tx + 64 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[i][g].x += x[i] * y.x; acc[i][g].y += x[i] * y.y; acc[i][g].z += x[i] * y.z; acc[i][g].w += x[i] * y.w;
+    for (int u = 0; u < 4; ++u) {
+      const float4 v = *reinterpret_cast<const float4*>(TRANSPOSED ? w + (n + u) * PITCH_S + 4 * ty : w + (4 * ty + u) * PITCH_S + n);
+      if constexpr (TRANSPOSED) {
+        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+      } else {
+        x[0][u] = v.x; x[1][u] = v.y; x[2][u] = v.z; x[3][u] = v.w;
       }
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int g = 0; g < HD / 64; ++g) {
+        const float4 y = *reinterpret_cast<const float4*>(b + (n + u) * (HD + 4) + 4 * tx + 64 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[i][g].x += x[u][i] * y.x; acc[i][g].y += x[u][i] * y.y; acc[i][g].z += x[u][i] * y.z; acc[i][g].w += x[u][i] * y.w;
+        }
+      }
   }
 }
 
@@ -76,7 +103,7 @@ __device__ __forceinline__ void store_rows(T* base, int64_t token_stride, const 
                                            const float (&factor)[4], int row0, int length, int dim, int ty, int tx) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = row0 + ty + 16 * i;
+    const int row = row0 + 4 * ty + i;
     if (row >= length) continue;
     T* dst = base + row * token_stride;
 #pragma unroll
@@ -138,7 +165,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const PlanRe
     tile_dot<HD>(s, qs, ks, ty, tx);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = row0 + ty + 16 * i;
+      const int row = row0 + 4 * ty + i;
       float best = top[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -156,7 +183,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const PlanRe
       for (int j = 0; j < 4; ++j) {
         const float p = s[i][j] == -INFINITY ? 0.0f : exp2f(s[i][j] - best);
         part += p;
-        ps[(ty + 16 * i) * PITCH_S + tx + 16 * j] = p;
+        ps[(4 * ty + i) * PITCH_S + tx + 16 * j] = p;
       }
 #pragma unroll
       for (int step = 8; step; step >>= 1) part += __shfl_xor_sync(0xffffffffu, part, step);
@@ -173,7 +200,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const PlanRe
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     factor[i] = 1.0f / sum[i];
-    const int row = row0 + ty + 16 * i;
+    const int row = row0 + 4 * ty + i;
     if (tx == 0 && row < r.length && a.lse) a.lse[(start + row) * a.heads + head] = top[i] + log2f(sum[i]);
   }
   T* out = static_cast<T*>(a.out) + (start * a.heads + head) * dim;
@@ -185,7 +212,7 @@ __device__ __forceinline__ void tile_slopes(float (&s)[4][4], float (&dp)[4][4],
                                             float scale, int row0, int key0, int length, int ty, int tx) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = row0 + ty + 16 * i;
+    const int row = row0 + 4 * ty + i;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int key = key0 + tx + 16 * j;
@@ -218,7 +245,7 @@ __global__ void __launch_bounds__(THREADS) attention_query_gradient_kernel(const
   float lse[4], delta[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = row0 + ty + 16 * i;
+    const int row = row0 + 4 * ty + i;
     lse[i] = row < r.length ? a.lse[(start + row) * a.heads + head] : 0.0f;
     delta[i] = row < r.length ? a.delta[(start + row) * a.heads + head] : 0.0f;
   }
@@ -237,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) attention_query_gradient_kernel(const
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ds[(ty + 16 * i) * PITCH_S + tx + 16 * j] = dp[i][j];
+      for (int j = 0; j < 4; ++j) ds[(4 * ty + i) * PITCH_S + tx + 16 * j] = dp[i][j];
     __syncthreads();
     tile_product<HD, false>(acc, ds, ks, ty, tx);
   }
@@ -278,7 +305,7 @@ __global__ void __launch_bounds__(THREADS) attention_key_gradient_kernel(const P
     float lse[4], delta[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = row0 + ty + 16 * i;
+      const int row = row0 + 4 * ty + i;
       lse[i] = row < r.length ? a.lse[(start + row) * a.heads + head] : 0.0f;
       delta[i] = row < r.length ? a.delta[(start + row) * a.heads + head] : 0.0f;
     }
@@ -291,8 +318,8 @@ __global__ void __launch_bounds__(THREADS) attention_key_gradient_kernel(const P
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        ps[(ty + 16 * i) * PITCH_S + tx + 16 * j] = s[i][j];
-        ds[(ty + 16 * i) * PITCH_S + tx + 16 * j] = dp[i][j];
+        ps[(4 * ty + i) * PITCH_S + tx + 16 * j] = s[i][j];
+        ds[(4 * ty + i) * PITCH_S + tx + 16 * j] = dp[i][j];
       }
     __syncthreads();
     tile_product<HD, true>(dv, ps, gs, ty, tx);
@@ -329,18 +356,30 @@ __global__ void attention_sum_heads_kernel(const PlanRecord* tiles, AttentionArg
   }
 }
 
-// delta[token, head] = sum over channels of dy * y; one warp per (token, head) row of the contiguous matrices.
-template <typename T>
-__global__ void attention_delta_kernel(const T* dy, const T* y, float* delta, int64_t rows, int dim) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; row < rows;
-       row += (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5) {
-    float sum = 0.0f;
-    for (int c = lane; c < dim; c += 32) sum += to_float<T>(dy[row * dim + c]) * to_float<T>(y[row * dim + c]);
+// delta[row] = sum over the channels of dy * y, rows = (token, head) of the contiguous matrices. A row is shared by LANES
+// lanes with 16 bytes each (VECTOR: rows are whole numbers of 16-byte pieces), or by a warp, element by element.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(256) attention_delta_kernel(const T* dy, const T* y, float* delta, int64_t rows, int dim, int lanes) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t row = thread / lanes;
+  const int lane = static_cast<int>(thread % lanes);
+  float sum = 0.0f;
+  if (row < rows) {
+    if constexpr (VECTOR) {
+      if (lane * N < dim) {
+        const uint4 a = *reinterpret_cast<const uint4*>(dy + row * dim + lane * N), b = *reinterpret_cast<const uint4*>(y + row * dim + lane * N);
+        const T* x = reinterpret_cast<const T*>(&a);
+        const T* z = reinterpret_cast<const T*>(&b);
 #pragma unroll
-    for (int step = 16; step; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
-    if (lane == 0) delta[row] = sum;
+        for (int i = 0; i < N; ++i) sum += to_float<T>(x[i]) * to_float<T>(z[i]);
+      }
+    } else {
+      for (int c = lane; c < dim; c += lanes) sum += to_float<T>(dy[row * dim + c]) * to_float<T>(y[row * dim + c]);
+    }
   }
+  for (int step = lanes / 2; step; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+  if (lane == 0 && row < rows) delta[row] = sum;
 }
 
 // Zeros for the tokens between documents: up to three matrices of `bytes[i]` per token, a multiple of 2.
@@ -362,26 +401,32 @@ int clear_gaps(const AttentionArgs& a, const GapTargets& t, int targets, cudaStr
   return check_launch("attention_clear_gaps_kernel");
 }
 
-template <typename Kernel, typename... Args>
-int launch(const char* name, Kernel kernel, dim3 grid, size_t smem, cudaStream_t stream, Args... args) {
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return fail(CT_ERR_CUDA, "%s: %s", name, cudaGetErrorString(err));
-  kernel<<<grid, THREADS, smem, stream>>>(args...);
+template <auto Kernel, typename... Args>
+int launch(const char* name, dim3 grid, int smem, cudaStream_t stream, Args... args) {
+  static DynamicSmem allowed;
+  const int rc = allowed.set(name, reinterpret_cast<const void*>(Kernel), smem);
+  if (rc) return rc;
+  Kernel<<<grid, THREADS, smem, stream>>>(args...);
   count_launch(false);
   return check_launch(name);
 }
 
 template <typename T, int HD> int simt_forward(const AttentionArgs& a, cudaStream_t stream) {
-  const size_t smem = (3 * TILE * (HD + 4) + TILE * PITCH_S) * sizeof(float);
-  return launch("attention_forward_kernel", attention_forward_kernel<T, HD>,
-                dim3(2 * a.count[kPlanTiles], a.heads), smem, stream, section(a, kPlanTiles), a);
+  const int smem = (3 * TILE * (HD + 4) + TILE * PITCH_S) * sizeof(float);
+  return launch<attention_forward_kernel<T, HD>>("attention_forward_kernel", dim3(2 * a.count[kPlanTiles], a.heads), smem, stream, section(a, kPlanTiles), a);
 }
 
 template <typename T> int delta_pass(const AttentionArgs& a, cudaStream_t stream) {
   const int64_t rows = a.tokens * a.heads;
-  const int64_t blocks = (rows + 7) / 8;
-  attention_delta_kernel<T><<<static_cast<unsigned>(blocks < 1 << 20 ? blocks : 1 << 20), 256, 0, stream>>>(
-      static_cast<const T*>(a.dy), static_cast<const T*>(a.out), a.delta, rows, a.head_dim);
+  const bool vector = a.head_dim * sizeof(T) % 16 == 0 && ((reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0;
+  int lanes = 32;
+  while (vector && lanes > 1 && (lanes / 2) * 16 >= a.head_dim * static_cast<int>(sizeof(T))) lanes /= 2;
+  const int64_t blocks = (rows * lanes + 255) / 256;
+  if (blocks > 0x7fffffff) return fail(CT_ERR_UNSUPPORTED, "ct_attention_backward: %lld rows", (long long)rows);
+  const T* dy = static_cast<const T*>(a.dy);
+  const T* y = static_cast<const T*>(a.out);
+  if (vector) attention_delta_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(dy, y, a.delta, rows, a.head_dim, lanes);
+  else attention_delta_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(dy, y, a.delta, rows, a.head_dim, lanes);
   count_launch(false);
   return check_launch("attention_delta_kernel");
 }
@@ -389,15 +434,15 @@ template <typename T> int delta_pass(const AttentionArgs& a, cudaStream_t stream
 template <typename T, int HD> int simt_backward(const AttentionArgs& a, cudaStream_t stream) {
   const dim3 grid(2 * a.count[kPlanTiles], a.heads);
   const PlanRecord* tiles = section(a, kPlanTiles);
-  const size_t query_smem = (4 * TILE * (HD + 4) + TILE * PITCH_S) * sizeof(float);
-  const size_t key_smem = query_smem + TILE * PITCH_S * sizeof(float);
-  int rc = launch("attention_query_gradient_kernel", attention_query_gradient_kernel<T, HD>, grid, query_smem, stream, tiles, a);
+  const int query_smem = (4 * TILE * (HD + 4) + TILE * PITCH_S) * sizeof(float);
+  const int key_smem = query_smem + TILE * PITCH_S * sizeof(float);
+  int rc = launch<attention_query_gradient_kernel<T, HD>>("attention_query_gradient_kernel", grid, query_smem, stream, tiles, a);
   if (rc) return rc;
   if (a.heads == a.kv_heads)
-    return launch("attention_key_gradient_kernel", attention_key_gradient_kernel<T, HD, false>, grid, key_smem, stream, tiles, a);
-  rc = launch("attention_key_gradient_kernel", attention_key_gradient_kernel<T, HD, true>, grid, key_smem, stream, tiles, a);
+    return launch<attention_key_gradient_kernel<T, HD, false>>("attention_key_gradient_kernel", grid, key_smem, stream, tiles, a);
+  rc = launch<attention_key_gradient_kernel<T, HD, true>>("attention_key_gradient_kernel", grid, key_smem, stream, tiles, a);
   if (rc) return rc;
-  return launch("attention_sum_heads_kernel", attention_sum_heads_kernel<T>, dim3(grid.x, a.kv_heads, 2), 0, stream, tiles, a);
+  return launch<attention_sum_heads_kernel<T>>("attention_sum_heads_kernel", dim3(grid.x, a.kv_heads, 2), 0, stream, tiles, a);
 }
 
 template <typename T> int simt_pass(const AttentionArgs& a, bool backward, cudaStream_t stream) {

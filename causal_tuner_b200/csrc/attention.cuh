@@ -2,9 +2,26 @@
 // tensor-core kernels (attention_tc.cu).
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ct {
+
+// The dynamic shared memory a kernel may use is raised once per device (a driver call of a microsecond otherwise).
+struct DynamicSmem {
+  std::atomic<uint64_t> done{0};
+  int set(const char* name, const void* kernel, int bytes) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    const uint64_t bit = 1ull << (device & 63);
+    if (err == cudaSuccess && (done.load(std::memory_order_relaxed) & bit)) return CT_OK;
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err != cudaSuccess) return fail(CT_ERR_CUDA, "%s: %s", name, cudaGetErrorString(err));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return CT_OK;
+  }
+};
 
 // A plan record: one tile of one document. `start` is the document's first token in the flattened batch, `length`
 // its token count, `a` and `b` depend on the section (include/ct_b200.h).

@@ -256,7 +256,7 @@ template <int HD> struct ForwardShape {
   static constexpr int kBoxes = HD / 64;
   static constexpr uint32_t kTile = kBoxes * BOX_BYTES;
   static constexpr int kRing = 2;
-  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + 1024 + 256;
+  static constexpr int kSmem = (2 + 2 * kRing) * kTile + 1024 + 256;
 };
 // Three warpgroups: two own a stage each, the third holds the copy and the MMA warp (two of its warps idle). Launched
 // with 168 registers a thread; the third hands down registers so that a thread can hold a row of 128 scores:
@@ -562,7 +562,7 @@ template <int HD> struct KeyShape {
   static constexpr int kRing = 2;
   static constexpr uint32_t kStatTile = 128 * 32;                // 128 rows x 16 values
   static constexpr uint32_t kStats = 2 * kStatTile;              // log-sums, deltas
-  static constexpr size_t kSmem = (2 + 2 * kRing) * kTile + kStatTile + kRing * kStats + 1024 + 256;
+  static constexpr int kSmem = (2 + 2 * kRing) * kTile + kStatTile + kRing * kStats + 1024 + 256;
 };
 
 // The statistics of a query tile vary along the COLUMNS of the transposed score tile, so every thread would need all of
@@ -864,25 +864,24 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
   if (warp == 9) tmem_free(tmem);
 }
 
-// dk (z = 0) and dv (z = 1) of the key tiles that were cut into pieces: the pieces' shares added in order.
+// dk and dv of the key tiles that were cut into pieces: the pieces' shares added in order, four channels per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) attention_sum_pieces_kernel(const __grid_constant__ AttentionParams p) {
   const PlanRecord r = p.items[blockIdx.x];            // (first token, rows, first slot, slots)
-  const int shared = blockIdx.y, which = blockIdx.z, quads = p.dim / 4;
-  T* out = static_cast<T*>(which ? p.dv : p.dk);
+  const int shared = blockIdx.z / 2, which = blockIdx.z % 2, quads = p.dim / 4;
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= r.length * quads) return;
   const int64_t step = static_cast<int64_t>(p.kv_heads) * 2 * 128 * p.dim;
-  const float* base = p.partials + ((static_cast<int64_t>(r.a) * p.kv_heads + shared) * 2 + which) * 128 * p.dim;
-  for (int i = threadIdx.x; i < r.length * quads; i += 256) {
-    const float* src = base + 4 * i;
-    float4 sum = *reinterpret_cast<const float4*>(src);
-    for (int s = 1; s < r.b; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(src + s * step);
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-    }
-    const int row = i / quads, at = 4 * (i % quads);
-    *reinterpret_cast<uint2*>(out + ((static_cast<int64_t>(r.start) + row) * p.kv_heads + shared) * p.dim + at) =
-        make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
+  const float* src = p.partials + ((static_cast<int64_t>(r.a) * p.kv_heads + shared) * 2 + which) * 128 * p.dim + 4 * i;
+  float4 sum = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+  for (int s = 1; s < r.b; ++s) {
+    const float4 v = __ldcs(reinterpret_cast<const float4*>(src + s * step));
+    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
+  const int row = i / quads, at = 4 * (i % quads);
+  *reinterpret_cast<uint2*>(static_cast<T*>(which ? p.dv : p.dk) + ((static_cast<int64_t>(r.start) + row) * p.kv_heads + shared) * p.dim + at) =
+      make_uint2(pack2<T>(sum.x, sum.y), pack2<T>(sum.z, sum.w));
 }
 
 // dq of one 128-row tile over the document's keys: S = Q K^T, dP = dY V^T, dQ += dS K. A thread owns a row (two
@@ -892,7 +891,7 @@ __global__ void __launch_bounds__(256) attention_sum_pieces_kernel(const __grid_
 template <int HD> struct QueryShape {
   static constexpr uint32_t kTile = HD / 64 * BOX_BYTES;
   static constexpr int kKeyRing = 3, kValueRing = 2;
-  static constexpr size_t kSmem = (2 + kKeyRing + kValueRing) * kTile + 1024 + 256;
+  static constexpr int kSmem = (2 + kKeyRing + kValueRing) * kTile + 1024 + 256;
 };
 
 template <typename T, int HD>
@@ -1156,18 +1155,19 @@ int fill(AttentionParams& p, const AttentionArgs& a, PlanSection which) {
   return rc;
 }
 
-int launch_tc(const char* name, void (*kernel)(AttentionParams), const AttentionParams& p, int64_t blocks, int threads, size_t smem,
-              cudaStream_t stream) {
+template <auto Kernel>
+int launch_tc(const char* name, const AttentionParams& p, int64_t blocks, int threads, int smem, cudaStream_t stream) {
   if (blocks > 0x7fffffff) return fail(CT_ERR_UNSUPPORTED, "%s: %lld blocks", name, (long long)blocks);
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err != cudaSuccess) return fail(CT_ERR_CUDA, "%s: %s", name, cudaGetErrorString(err));
-  kernel<<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
+  static DynamicSmem allowed;
+  const int rc = allowed.set(name, reinterpret_cast<const void*>(Kernel), smem);
+  if (rc) return rc;
+  Kernel<<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
   count_launch(true);
   return check_launch(name);
 }
 
 template <typename T, int HD> int forward(const AttentionArgs& a, const AttentionParams& p, cudaStream_t stream) {
-  return launch_tc("attention_forward_tc_kernel", attention_forward_tc_kernel<T, HD>, p, a.count[kPlanForward] * p.head_blocks,
+  return launch_tc<attention_forward_tc_kernel<T, HD>>("attention_forward_tc_kernel", p, a.count[kPlanForward] * p.head_blocks,
                    kForwardThreads, ForwardShape<HD>::kSmem, stream);
 }
 
@@ -1180,15 +1180,17 @@ template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t 
   p.dk = a.dk;
   p.dv = a.dv;
   p.out = a.dq;
-  rc = launch_tc("attention_query_gradient_tc_kernel", attention_query_gradient_tc_kernel<T, HD>, p,
+  rc = launch_tc<attention_query_gradient_tc_kernel<T, HD>>("attention_query_gradient_tc_kernel", p,
                  a.count[kPlanQuery] * p.head_blocks, kBackwardThreads, QueryShape<HD>::kSmem, stream);
   if (rc) return rc;
   p.items = section(a, kPlanKeys);
-  rc = launch_tc("attention_key_gradient_tc_kernel", attention_key_gradient_tc_kernel<T, HD>, p, a.count[kPlanKeys] * p.kv_heads,
+  rc = launch_tc<attention_key_gradient_tc_kernel<T, HD>>("attention_key_gradient_tc_kernel", p, a.count[kPlanKeys] * p.kv_heads,
                  kBackwardThreads, KeyShape<HD>::kSmem, stream);
   if (rc || !a.count[kPlanReduce]) return rc;
   p.items = section(a, kPlanReduce);
-  attention_sum_pieces_kernel<T><<<dim3(a.count[kPlanReduce], a.kv_heads, 2), 256, 0, stream>>>(p);
+  if (a.kv_heads > 32767) return fail(CT_ERR_UNSUPPORTED, "ct_attention_backward: %d key heads", a.kv_heads);
+  const dim3 grid(a.count[kPlanReduce], (128 * a.head_dim / 4 + 255) / 256, 2 * a.kv_heads);
+  attention_sum_pieces_kernel<T><<<grid, 256, 0, stream>>>(p);
   count_launch(false);
   return check_launch("attention_sum_pieces_kernel");
 }

@@ -7,7 +7,7 @@
 // tokens touch a quarter. So nothing is cleared beforehand and nothing is accumulated in memory: the tokens are sorted by id
 // (stable radix sort, a few us), every row knows its run of tokens and one kernel writes zeros, single rows and sums.
 // Sums are taken in token order in fp32 by the thread that owns the column: no atomics, repeated calls are bit-identical.
-// A run of more than 128 tokens (frequent tokens of a text) would keep one block busy, so runs are cut at multiples of 128
+// A run of more than 32 tokens (frequent tokens of a text) would keep one block busy, so runs are cut at multiples of 32
 // in the sorted order; the pieces of long runs are summed first, by as many blocks, and then added in order.
 #include "common.cuh"
 
@@ -17,8 +17,8 @@ namespace {
 constexpr int kRadixBits = 8, kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kBlockItems = 4 * kSortThreads;          // sorted by one block of the many-block sort
-constexpr int kOneBlockItems = 16 * kSortThreads;      // up to here one block sorts alone, in shared memory, in one launch
-constexpr int kPiece = 128;                            // sorted tokens per piece of a long run
+constexpr int kOneBlockItems = 4 * kSortThreads;       // up to here one block sorts alone, in shared memory, in one launch
+constexpr int kPiece = 32;                             // sorted tokens per piece of a long run
 constexpr int kBadToken = 9;                           // device error code
 
 // ---- forward ---------------------------------------------------------------------------
@@ -33,6 +33,11 @@ template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const
 #pragma unroll
     for (int e = 0; e < N; ++e) x[N * i + e] = to_float<T>(w.v[e]);
   }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {      // one 32-byte store
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   constexpr int N = 16 / sizeof(T);
@@ -59,7 +64,7 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const int64_t* i
       if (known) load8<W>(x, table + id * width + column);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= scale;
-      store8<T>(out + token * width + column, x);
+      store8(out + token * width + column, x);
     } else {
       out[token * width + column] = from_float<T>(known ? to_float<W>(table[id * width + column]) * scale : 0.0f);
     }
@@ -74,8 +79,17 @@ struct SortShared {
   int digit_base[kRadix];
 };
 
-// Lanes of the warp whose digit equals this lane's; inactive items have digit -1 and match each other only.
-__device__ __forceinline__ uint32_t same_digit(int digit) { return __match_any_sync(0xffffffffu, digit); }
+// Lanes of the warp whose digit equals this lane's, among lanes with an item (digit >= 0). A vote per bit: the match
+// instruction made the one-block sort of 16384 tokens take 81 us.
+__device__ __forceinline__ uint32_t same_digit(int digit) {
+  uint32_t peers = __ballot_sync(0xffffffffu, digit >= 0);
+#pragma unroll
+  for (int bit = 0; bit < kRadixBits; ++bit) {
+    const uint32_t ones = __ballot_sync(0xffffffffu, (digit >> bit) & 1);
+    peers &= (digit >> bit) & 1 ? ones : ~ones;
+  }
+  return peers;
+}
 
 template <int STEPS> __device__ __forceinline__ void count_digits(SortShared& s, const int (&digit)[STEPS]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,36 +166,36 @@ __device__ __forceinline__ int item_index(int k, int items_per_warp) {
   return (threadIdx.x >> 5) * items_per_warp + 32 * k + (threadIdx.x & 31);
 }
 
-constexpr int kOneBlockSteps = kOneBlockItems / kSortThreads;
+template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_block_kernel(const int64_t* ids, int tokens, int64_t rows, int64_t padding,
                                                                                 int bits, int* keys, int* positions, int* error_flag) {
-  extern __shared__ int2 items[];                       // (key, position), kOneBlockItems
+  extern __shared__ int2 items[];                       // (key, position)
   __shared__ SortShared s;
-  int2 mine[kOneBlockSteps];
-  int digit[kOneBlockSteps];
+  int2 mine[STEPS];
+  int digit[STEPS];
 #pragma unroll
-  for (int k = 0; k < kOneBlockSteps; ++k) {
-    const int at = item_index(k, kOneBlockItems / kSortWarps);
+  for (int k = 0; k < STEPS; ++k) {
+    const int at = item_index(k, 32 * STEPS);
     mine[k] = at < tokens ? make_int2(key_of(ids[at], rows, padding, error_flag), at) : make_int2(-1, 0);
   }
   for (int shift = 0; shift < bits; shift += kRadixBits) {
 #pragma unroll
-    for (int k = 0; k < kOneBlockSteps; ++k) digit[k] = mine[k].x < 0 ? -1 : (mine[k].x >> shift) & (kRadix - 1);
+    for (int k = 0; k < STEPS; ++k) digit[k] = mine[k].x < 0 ? -1 : (mine[k].x >> shift) & (kRadix - 1);
     count_digits(s, digit);
     const int total = sum_over_warps(s);
     digit_sums(s, total);
     hand_out(s, digit, [&](int k, int at) { items[at] = mine[k]; });
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kOneBlockSteps; ++k) {
-      const int at = item_index(k, kOneBlockItems / kSortWarps);
+    for (int k = 0; k < STEPS; ++k) {
+      const int at = item_index(k, 32 * STEPS);
       mine[k] = at < tokens ? items[at] : make_int2(-1, 0);
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int k = 0; k < kOneBlockSteps; ++k) {
-    const int at = item_index(k, kOneBlockItems / kSortWarps);
+  for (int k = 0; k < STEPS; ++k) {
+    const int at = item_index(k, 32 * STEPS);
     if (at < tokens) {
       keys[at] = mine[k].x;
       positions[at] = mine[k].y;
@@ -214,32 +228,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_count_kernel(cons
   for (int k = 0; k < kBlockSteps; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
   count_digits(s, digit);
   const int total = sum_over_warps(s);
-  if (threadIdx.x < kRadix) histogram[static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x] = total;
-}
-
-// Exclusive sums over `count` values in place, by one block.
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_scan_kernel(int* values, int64_t count) {
-  __shared__ int warp_sum[kSortWarps];
-  __shared__ int carry;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) carry = 0;
-  for (int64_t first = 0; first < count; first += kSortThreads) {
-    const int64_t at = first + threadIdx.x;
-    const int value = at < count ? values[at] : 0;
-    int inclusive = value;
-#pragma unroll
-    for (int step = 1; step < 32; step <<= 1) {
-      const int other = __shfl_up_sync(0xffffffffu, inclusive, step);
-      if (lane >= step) inclusive += other;
-    }
-    if (lane == 31) warp_sum[warp] = inclusive;
-    __syncthreads();
-    int before = carry;
-    for (int w = 0; w < warp; ++w) before += warp_sum[w];
-    if (at < count) values[at] = before + inclusive - value;
-    __syncthreads();
-    if (threadIdx.x == kSortThreads - 1) carry = before + inclusive;
-  }
+  if (threadIdx.x < kRadix) histogram[static_cast<int64_t>(blockIdx.x) * kRadix + threadIdx.x] = total;
 }
 
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(const int64_t* ids, const int* src_keys, const int* src_positions,
@@ -252,7 +241,16 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(co
   for (int k = 0; k < kBlockSteps; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
   count_digits(s, digit);
   sum_over_warps(s);
-  if (threadIdx.x < kRadix) s.digit_base[threadIdx.x] = histogram[static_cast<int64_t>(threadIdx.x) * gridDim.x + blockIdx.x];
+  // every block sums the histogram for itself: the digit's items in all blocks, and in the blocks before this one
+  int total = 0, before = 0;
+  if (threadIdx.x < kRadix)
+    for (unsigned b = 0; b < gridDim.x; ++b) {
+      const int n = histogram[static_cast<int64_t>(b) * kRadix + threadIdx.x];
+      before += b < blockIdx.x ? n : 0;
+      total += n;
+    }
+  digit_sums(s, total);
+  if (threadIdx.x < kRadix) s.digit_base[threadIdx.x] += before;
   __syncthreads();
   hand_out(s, digit, [&](int k, int at) {
     keys[at] = key[k];
@@ -294,17 +292,17 @@ __device__ __forceinline__ void load_columns(float (&x)[N], const T* p) {
   else x[0] = to_float<T>(*p);
 }
 
-// sum += dy[positions[i]] for i in [first, last), in order; four rows in flight.
+// sum += dy[positions[i]] for i in [first, last), in order; eight rows in flight.
 template <typename T, bool VECTOR, int N = VECTOR ? 8 : 1>
 __device__ __forceinline__ void add_rows(float (&sum)[N], const GradientArgs& a, int first, int last, int64_t column) {
   const T* dy = static_cast<const T*>(a.dy) + column;
   int i = first;
-  for (; i + 4 <= last; i += 4) {
-    float x[4][N];
+  for (; i + 8 <= last; i += 8) {
+    float x[8][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load_columns<T, VECTOR>(x[u], dy + a.positions[i + u] * a.ld);
+    for (int u = 0; u < 8; ++u) load_columns<T, VECTOR>(x[u], dy + a.positions[i + u] * a.ld);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 8; ++u)
 #pragma unroll
       for (int e = 0; e < N; ++e) sum[e] += x[u][e];
   }
@@ -335,6 +333,10 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int
   for (int which = 0; which < 2; ++which) {
     const int key = which ? tail : head;
     if (key >= a.rows || (which && tail == head)) continue;
+    // a run that neither reaches in nor reaches out is not a long one
+    const bool reaches_in = !which && begin > 0 && a.keys[begin - 1] == key;
+    const bool reaches_out = key == tail && end < tokens && a.keys[end] == key;
+    if (!reaches_in && !reaches_out) continue;
     const int first = lower_bound(a.keys, tokens, key), last = lower_bound(a.keys, tokens, key + 1);
     if (last - first <= kPiece || column >= a.width) continue;
     float sum[N] = {};
@@ -345,19 +347,34 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int
   }
 }
 
-// Every row of the table, every column: zeros, or the sum of the row's run.
+// Every row of the table, every column: zeros, or the sum of the row's run. A block takes kRowsPerBlock rows so that the
+// (dependent) load of where their runs start is paid once: 141 us instead of 204 with a row per block, 16384 tokens on
+// 49152 x 4096.
+constexpr int kRowsPerBlock = 8;
 template <typename T, typename W, bool VECTOR>
 __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a) {
   constexpr int N = VECTOR ? 8 : 1;
   const int64_t column = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * N;
+  if (column >= a.width) return;
   W* out = static_cast<W*>(a.out) + column;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int first = a.starts[row], last = a.starts[row + 1];
-    if (column >= a.width) continue;
+  // rows a grid's width apart: frequent tokens tend to be neighbours and should not meet in one block
+  int starts[kRowsPerBlock], ends[kRowsPerBlock];
+#pragma unroll
+  for (int r = 0; r < kRowsPerBlock; ++r) {
+    const int64_t row = blockIdx.x + static_cast<int64_t>(r) * gridDim.x;
+    starts[r] = row < a.rows ? a.starts[row] : 0;
+    ends[r] = row < a.rows ? a.starts[row + 1] : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < kRowsPerBlock; ++r) {
+    const int first = starts[r], last = ends[r];
+    const int64_t row = blockIdx.x + static_cast<int64_t>(r) * gridDim.x;
+    if (row >= a.rows) break;
     float sum[N] = {};
     if (last - first <= kPiece) {
       add_rows<T, VECTOR>(sum, a, first, last, column);
     } else {
+#pragma unroll 4
       for (int piece = first / kPiece; piece * kPiece < last; ++piece) {
         // the run fills the piece's first place unless it begins inside the piece, behind another run
         const int which = first > piece * kPiece ? 1 : 0;
@@ -368,7 +385,7 @@ __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a)
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) sum[e] *= a.scale;
-    if constexpr (VECTOR) store8<W>(out + row * a.width, sum);
+    if constexpr (VECTOR) store8(out + row * a.width, sum);
     else out[row * a.width] = from_float<W>(sum[0]);
   }
 }
@@ -396,10 +413,14 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
                 int* other_positions, int* histogram, int* error_flag, cudaStream_t stream) {
   const int bits = bits_of(rows), passes = (bits + kRadixBits - 1) / kRadixBits;
   if (tokens <= kOneBlockItems) {
-    const size_t smem = kOneBlockItems * sizeof(int2);
-    const cudaError_t err = cudaFuncSetAttribute(embedding_sort_one_block_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // 1 or 4 tokens a thread (with 16, one block takes 51 us for 16384 tokens, many blocks half of that)
+    const int steps = tokens <= kSortThreads ? 1 : 4;
+    const auto kernel = steps == 1 ? embedding_sort_one_block_kernel<1> : embedding_sort_one_block_kernel<4>;
+    const int smem = steps * kSortThreads * static_cast<int>(sizeof(int2));
+    // with the 33 KB of counters all but the smallest are above the default limit
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return fail(CT_ERR_CUDA, "embedding_sort_one_block_kernel: %s", cudaGetErrorString(err));
-    embedding_sort_one_block_kernel<<<1, kSortThreads, smem, stream>>>(ids, static_cast<int>(tokens), rows, padding, bits, keys, positions, error_flag);
+    kernel<<<1, kSortThreads, smem, stream>>>(ids, static_cast<int>(tokens), rows, padding, bits, keys, positions, error_flag);
     count_launch(false);
     return check_launch("embedding_sort_one_block_kernel");
   }
@@ -412,10 +433,9 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
     int* to_positions = last_is_first ? positions : other_positions;
     const int shift = pass * kRadixBits;
     embedding_sort_count_kernel<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
-    embedding_sort_scan_kernel<<<1, kSortThreads, 0, stream>>>(histogram, static_cast<int64_t>(kRadix) * blocks);
     embedding_sort_scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, from_positions, tokens, rows, padding, shift, histogram,
                                                                        to_keys, to_positions, error_flag);
-    for (int i = 0; i < 3; ++i) count_launch(false);
+    for (int i = 0; i < 2; ++i) count_launch(false);
     from_keys = to_keys;
     from_positions = to_positions;
   }
@@ -432,7 +452,7 @@ template <typename T, typename W, bool VECTOR> int gradient(const GradientArgs& 
   count_launch(false);
   const int rc = check_launch("embedding_runs_kernel");
   if (rc) return rc;
-  const int64_t grid = a.rows < (1 << 20) ? a.rows : 1 << 20;
+  const int64_t grid = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock;
   embedding_gradient_kernel<T, W, VECTOR><<<dim3(static_cast<unsigned>(grid), static_cast<unsigned>(column_blocks)), 256, 0, stream>>>(a);
   count_launch(false);
   return check_launch("embedding_gradient_kernel");

@@ -131,22 +131,24 @@ def _check(q, k, v, plan):
 
 
 def _rows(tensor):
-    """The tensor as [tokens, heads, head_dim] with contiguous channels, copied only where the strides demand it."""
-    flat = tensor.flatten(0, 1)
-    if flat.stride(2) != 1 and flat.shape[2] > 1 or any(s <= 0 for s, n in zip(flat.stride(), flat.shape) if n > 1):
-        flat = flat.contiguous()
-    return flat
+    """(tensor, token stride, head stride) of [rows, width, heads, head_dim] as [tokens, heads, head_dim] with contiguous
+    channels, copied only where the strides demand it; strides of dimensions of one element are made regular."""
+    rows, width, heads, dim = tensor.shape
+    if not tensor.is_contiguous():
+        row, token, head, channel = tensor.stride()
+        if ((channel != 1 and dim > 1) or (rows > 1 and width > 1 and row != width * token) or (heads > 1 and head <= 0)
+                or (width > 1 and token <= 0) or (rows > 1 and row <= 0)):
+            tensor = tensor.contiguous()
+        else:
+            head = head if heads > 1 else dim
+            return tensor, token if width > 1 else row if rows > 1 else heads * head, head
+    return tensor, heads * dim, dim
 
 
 def _operands(*tensors):
-    """(pointer, token stride, head stride) of each; the strides of dimensions of one element are made regular."""
-    result = []
-    for tensor in tensors:
-        tokens, heads, dim = tensor.shape
-        head_stride = tensor.stride(1) if heads > 1 else dim
-        token_stride = tensor.stride(0) if tokens > 1 else heads * head_stride
-        result += [tensor.data_ptr(), token_stride, head_stride]
-    return result
+    """The (copied where necessary) tensors, and (pointer, token stride, head stride) of each."""
+    views = [_rows(tensor) for tensor in tensors]
+    return [view[0] for view in views], [n for tensor, *strides in views for n in (tensor.data_ptr(), *strides)]
 
 
 def _aligned(tensor):
@@ -159,13 +161,14 @@ def attention_forward(q, k, v, plan, *, scale=None, keep_lse=True):
     """(y, lse): the attention output, shaped like q, and the rows' base-2 log-sums [tokens, heads] (None without
     `keep_lse`). `scale` defaults to head_dim ** -0.5."""
     _check(q, k, v, plan)
-    rows = [_rows(t) for t in (q, k, v)]
-    tokens, heads, dim = rows[0].shape
+    rows, width, heads, dim = q.shape
+    tokens = rows * width
+    kept, operands = _operands(q, k, v)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     lse = torch.empty((tokens, heads), device=q.device, dtype=torch.float32) if keep_lse else None
     if out.numel() == 0:
         return out, lse
-    library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
+    library, code = _lib.load(), _lib.code_of(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q):
         path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
@@ -190,13 +193,14 @@ def attention_backward(dy, q, k, v, y, lse, plan, *, scale=None):
         raise ValueError("dy, y and lse must be on the device of q")
     if lse.shape != (q.shape[0] * q.shape[1], q.shape[2]) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be the contiguous fp32 [tokens, heads] of the forward pass")
-    rows = [_rows(t) for t in (q, k, v)]
+    rows, width, heads, dim = q.shape
+    tokens = rows * width
+    kept, operands = _operands(q, k, v)
     dy, y = _aligned(dy.to(q.dtype)), _aligned(y.to(q.dtype))
-    tokens, heads, dim = rows[0].shape
     dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
     if dq.numel() == 0:
         return dq, dk, dv
-    library, operands, code = _lib.load(), _operands(*rows), _lib.code_of(q.dtype)
+    library, code = _lib.load(), _lib.code_of(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q):
         path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
@@ -229,4 +233,6 @@ class DocumentAttention(torch.autograd.Function):
 def document_attention(q, k, v, plan, *, scale=None):
     """Causal attention inside the plan's documents: q [rows, width, heads, head_dim], k and v
     [rows, width, kv_heads, head_dim] -> shaped like q, differentiable in all three."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return attention_forward(q, k, v, plan, scale=scale, keep_lse=False)[0]
     return DocumentAttention.apply(q, k, v, plan, scale)

@@ -81,4 +81,6 @@ class Embedding(torch.autograd.Function):
 
 def embed_tokens(ids, weight, *, scale=1.0, dtype=None, padding_idx=None):
     """`embedding_lookup`, differentiable in `weight`; `padding_idx` is the row that gets no gradient."""
+    if not (torch.is_grad_enabled() and weight.requires_grad):
+        return embedding_lookup(ids, weight, scale=scale, dtype=dtype)
     return Embedding.apply(weight, ids, float(scale), dtype, padding_idx)

@@ -513,7 +513,7 @@ CT_API int ct_attention_backward(const void* q, int64_t q_token, int64_t q_head,
  * backward pass when the embedding trains (modeling/model.py:185-193).
  * ct_embedding_forward: out[t, :] = round(scale * table[ids[t], :]) in `out_dtype`; table [rows, width] contiguous.
  * ct_embedding_gradient: d_table[i, :] = scale * sum of dy[t, :] over the tokens with ids[t] == i, in fp32 in the order of
- *   t (runs of more than 128 tokens: pieces of the sorted order, added in order), rounded once to `table_dtype`; zero
+ *   t (runs of more than 32 tokens: pieces of the sorted order, added in order), rounded once to `table_dtype`; zero
  *   for every other row and for row `padding` (-1: none). The whole [rows, width] matrix is written. dy has `ld` elements
  *   between rows. No atomics: repeated calls are bit-identical.
  *   `workspace`: ct_embedding_gradient_workspace bytes, 256-byte aligned.

@@ -75,7 +75,7 @@ def test_gradient_scale_padding_and_table_types(table):
 
 
 def test_gradient_equals_the_sums_in_token_order():
-    """Runs of up to 128 tokens are plain fp32 sums in token order: integers show that every token is counted once."""
+    """Runs of up to 32 tokens are plain fp32 sums in token order: integers show that every token is counted once."""
     tokens, rows = 20000, 40000
     ids = make_ids(tokens, rows, "uniform")
     dy = torch.randint(-100, 100, (tokens, 16), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").float()

@@ -23,10 +23,10 @@ def test_entry_points_check_their_arguments():
 
 def test_workspace():
     size = _lib.load().ct_embedding_gradient_workspace
-    # two lists of 1000 tokens, 11 run starts, 8 pieces x 2 rows of 16 floats
-    assert size(1000, 10, 16) == 2 * 4096 + 256 + 1024
-    # above 16384 tokens four lists and the blocks' histograms
-    assert size(20000, 10, 16) == 4 * 80128 + 5 * 256 * 4 + 256 + 157 * 2 * 64 + 128
+    # two lists of 1000 tokens, 11 run starts, 32 pieces x 2 rows of 16 floats
+    assert size(1000, 10, 16) == 2 * 4096 + 256 + 4096
+    # above 4096 tokens four lists and the blocks' histograms
+    assert size(20000, 10, 16) == 4 * 80128 + 5 * 256 * 4 + 256 + 625 * 2 * 64 + 128
 
 
 def test_no_cpu_path():
