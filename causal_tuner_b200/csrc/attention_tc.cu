@@ -14,6 +14,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "attention.cuh"
@@ -207,6 +208,7 @@ struct AttentionParams {
   int heads, kv_heads, dim;
   int packed, tile_tokens; // packed * tile_tokens = 128
   int head_blocks;         // 128-row blocks of heads: heads / packed
+  int units;               // records x head blocks (key gradients: x key heads)
   float scale;
   int* error_flag;
 };
@@ -232,6 +234,12 @@ struct Waiter {
     }
     return true;
   }
+  // two barriers, by a whole warp: one round trip where both are complete
+  __device__ __forceinline__ bool both(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, int code) const {
+    const uint32_t first = mbar_try_wait(a, a_parity), second = mbar_try_wait(b, b_parity);
+    if (__all_sync(0xffffffffu, first & second)) return true;
+    return warp(a, a_parity, code) && warp(b, b_parity, code);
+  }
   // by a whole warp, which stays together
   __device__ __forceinline__ bool warp(uint32_t bar, uint32_t parity, int code) const {
     return __all_sync(0xffffffffu, (*this)(bar, parity, code));
@@ -244,6 +252,33 @@ __device__ __forceinline__ void settle(const volatile int* abort_flag) {
   const uint64_t start = global_timer_ns();
   while (global_timer_ns() - start < 1000000ull) __nanosleep(1000);
 }
+
+// The kernels are persistent, one CTA per SM: copies and first products of a CTA's next tile of queries (or keys) run
+// under the tail of the last one, which pays where documents are short (a CTA per tile spent 4 to 6 us on starting, the
+// first copies and the end, as much as 500 keys of work). Units are sorted by falling work and dealt back and forth, so
+// that the CTAs' sums come out even.
+__device__ __forceinline__ int unit_of_round(int round) {
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  return round * ctas + (round & 1 ? ctas - 1 - cta : cta);
+}
+
+// A CTA's walk over its units, `per_record` units to a record; the record after the current one is read ahead.
+struct Walk {
+  const PlanRecord* records;
+  int units, per_record, round, unit;
+  PlanRecord here, ahead;
+  __device__ __forceinline__ PlanRecord read(int u) const { return records[min(u, units - 1) / per_record]; }
+  __device__ __forceinline__ Walk(const PlanRecord* r, int n, int per) : records(r), units(n), per_record(per), round(0), unit(unit_of_round(0)) {
+    here = uniform(read(unit));
+    ahead = read(unit_of_round(1));
+  }
+  __device__ __forceinline__ bool valid() const { return unit < units; }
+  __device__ __forceinline__ void next() {
+    unit = unit_of_round(++round);
+    here = uniform(ahead);
+    ahead = read(unit_of_round(round + 1));
+  }
+};
 
 // ---- forward -------------------------------------------------------------------------
 // Two 128-row stages per CTA against one stream of key tiles; per stage and tile
@@ -894,6 +929,32 @@ template <int HD> struct QueryShape {
   static constexpr int kSmem = (2 + kKeyRing + kValueRing) * kTile + 1024 + 256;
 };
 
+// A tile of queries and its position among the document's keys, as the MMA warp walks them.
+struct QueryWalk : Walk {
+  int tile_tokens, head_blocks, group, packed;
+  int n, end, head0, shared, j;
+  __device__ __forceinline__ QueryWalk(const AttentionParams& p)
+      : Walk(p.items, p.units, p.head_blocks), tile_tokens(p.tile_tokens), head_blocks(p.head_blocks), group(p.heads / p.kv_heads), packed(p.packed) {
+    open();
+  }
+  __device__ __forceinline__ void open() {
+    head0 = unit % head_blocks * packed;
+    shared = head0 / group;
+    end = min(here.length, here.a + tile_tokens);                 // keys [0, end) are all the tile can see
+    n = (end + KEYS - 1) / KEYS;
+    j = 0;
+  }
+  __device__ __forceinline__ void next_unit() {
+    next();
+    open();
+  }
+  __device__ __forceinline__ void advance() {
+    if (++j == n) next_unit();
+  }
+  __device__ __forceinline__ bool last() const { return j + 1 == n; }
+  __device__ __forceinline__ int columns(int tile) const { return min(KEYS, (end - tile * KEYS + 31) & ~31); }
+};
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_tc_kernel(const __grid_constant__ AttentionParams p) {
   using Shape = QueryShape<HD>;
@@ -903,27 +964,25 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t q_tile = smem_u32(smem), g_tile = q_tile + TILE, k_ring = g_tile + TILE, v_ring = k_ring + KR * TILE;
   const uint32_t bars = v_ring + VR * TILE;
-  const uint32_t q_full = bars, g_full = bars + 8, dp_full = bars + 16, ds_ready = bars + 24, done = bars + 32;
-  auto s_full = [&](int b) { return bars + 40u + 8u * b; };
-  auto k_full = [&](int r) { return bars + 56u + 8u * r; };
-  auto k_empty = [&](int r) { return bars + 56u + 8u * (KR + r); };
-  auto v_full = [&](int r) { return bars + 56u + 8u * (2 * KR + r); };
-  auto v_empty = [&](int r) { return bars + 56u + 8u * (2 * KR + VR + r); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + KR + VR) * TILE + 56 + 16 * (KR + VR));
+  const uint32_t q_full = bars, g_full = bars + 8, dp_full = bars + 16, ds_ready = bars + 24, done = bars + 32, q_empty = bars + 40, g_empty = bars + 48;
+  auto s_full = [&](int b) { return bars + 56u + 8u * b; };
+  auto k_full = [&](int r) { return bars + 72u + 8u * r; };
+  auto v_full = [&](int r) { return bars + 72u + 8u * (KR + r); };
+  auto v_empty = [&](int r) { return bars + 72u + 8u * (KR + VR + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + KR + VR) * TILE + 72 + 8 * (KR + 2 * VR));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(g_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(g_empty, 1);
     mbar_init(dp_full, 1);
     mbar_init(ds_ready, 8);
     mbar_init(done, 1);
     for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1);
-    for (int r = 0; r < KR; ++r) {
-      mbar_init(k_full(r), 1);
-      mbar_init(k_empty(r), 1);
-    }
+    for (int r = 0; r < KR; ++r) mbar_init(k_full(r), 1);
     for (int r = 0; r < VR; ++r) {
       mbar_init(v_full(r), 1);
       mbar_init(v_empty(r), 1);
@@ -938,160 +997,190 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
   tcgen05_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
   const Waiter wait{abort_flag, p.error_flag};
-
-  const PlanRecord item = uniform(p.items[blockIdx.x / p.head_blocks]);
-  const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
-  const int shared = head0 / (p.heads / p.kv_heads);
-  const int end = min(item.length, item.a + p.tile_tokens);        // keys [0, end) are all this tile can see
-  const int n = (end + KEYS - 1) / KEYS;
-  auto columns = [&](int j) { return min(KEYS, (end - j * KEYS + 31) & ~31); };
+  // Tiles of keys are counted through all units (t): ring slots, S buffers and barrier phases go by t; those that are
+  // used once per unit go by the round.
 
   if (warp >= 8) {
     registers_down<104>();
     if (warp == 8) {
-      if (lane == 0) {
-        const int token = item.start + item.a;
-        mbar_expect_tx(q_full, TILE);
-        for (int b = 0; b < BOXES; ++b) tma_load_3d(q_tile + b * BOX_BYTES, &p.q, q_full, 64 * b, head0, token);
-        for (int j = 0; j < n; ++j) {
-          const int kr = j % KR, vr = j % VR;
-          if (!wait(k_empty(kr), ((j / KR) & 1) ^ 1, 6)) break;
-          mbar_expect_tx(k_full(kr), TILE);
-          for (int b = 0; b < BOXES; ++b) tma_load_3d(k_ring + kr * TILE + b * BOX_BYTES, &p.k, k_full(kr), 64 * b, shared, item.start + j * KEYS);
-          if (j == 0) {
-            mbar_expect_tx(g_full, TILE);
-            for (int b = 0; b < BOXES; ++b) tma_load_3d(g_tile + b * BOX_BYTES, &p.dy, g_full, 64 * b, head0, token);
+      bool alive = true;
+      int t = 0;
+      for (QueryWalk w(p); w.valid() && alive; w.next_unit()) {
+        const int token = w.here.start + w.here.a;
+        const uint32_t free_parity = (w.round & 1) ^ 1;
+        if (!wait.warp(q_empty, free_parity, 6)) break;
+        if (elect_one()) {
+          mbar_expect_tx(q_full, TILE);
+          for (int b = 0; b < BOXES; ++b) tma_load_3d(q_tile + b * BOX_BYTES, &p.q, q_full, 64 * b, w.head0, token);
+        }
+        for (int j = 0; j < w.n; ++j, ++t) {
+          const int kr = t % KR, vr = t % VR, key = w.here.start + j * KEYS;
+          // the slot's last tile, t - 3, was read by its dQ, and S(t - 1) was issued behind that (its next phase needs this
+          // tile, so the phase waited for cannot be missed)
+          if (t >= KR && !wait.warp(s_full((t - 1) & 1), ((t - 1) >> 1) & 1, 6)) { alive = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(k_full(kr), TILE);
+            for (int b = 0; b < BOXES; ++b) tma_load_3d(k_ring + kr * TILE + b * BOX_BYTES, &p.k, k_full(kr), 64 * b, w.shared, key);
           }
-          if (!wait(v_empty(vr), ((j / VR) & 1) ^ 1, 6)) break;
-          mbar_expect_tx(v_full(vr), TILE);
-          for (int b = 0; b < BOXES; ++b) tma_load_3d(v_ring + vr * TILE + b * BOX_BYTES, &p.v, v_full(vr), 64 * b, shared, item.start + j * KEYS);
+          if (j == 0) {
+            if (!wait.warp(g_empty, free_parity, 6)) { alive = false; break; }
+            if (elect_one()) {
+              mbar_expect_tx(g_full, TILE);
+              for (int b = 0; b < BOXES; ++b) tma_load_3d(g_tile + b * BOX_BYTES, &p.dy, g_full, 64 * b, w.head0, token);
+            }
+          }
+          if (!wait.warp(v_empty(vr), ((t / VR) & 1) ^ 1, 6)) { alive = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(v_full(vr), TILE);
+            for (int b = 0; b < BOXES; ++b) tma_load_3d(v_ring + vr * TILE + b * BOX_BYTES, &p.v, v_full(vr), 64 * b, w.shared, key);
+          }
         }
       }
-      __syncwarp();
     } else if (warp == 9) {
-      auto scores = [&](int j) {
-        product_nt<T, HD>(tmem + (j & 1) * 128, q_tile, k_ring + (j % KR) * TILE, columns(j));
-        commit(s_full(j & 1));
+      bool alive = true;
+      auto scores = [&](const QueryWalk& w, int t) {
+        alive = (w.j > 0 || wait.warp(q_full, w.round & 1, 7)) && wait.warp(k_full(t % KR), (t / KR) & 1, 7);
+        if (!alive) return;
+        product_nt<T, HD>(tmem + (t & 1) * 128, q_tile, k_ring + (t % KR) * TILE, w.columns(w.j));
+        commit(s_full(t & 1));
+        if (w.last()) commit(q_empty);
       };
-      auto slopes = [&](int j) {
-        product_nt<T, HD>(tmem + 256, g_tile, v_ring + (j % VR) * TILE, columns(j));
+      // a commit costs this warp 130 cycles: slots of the rings are released by who sees the products complete
+      auto slopes = [&](const QueryWalk& w, int t) {
+        if (w.j == 0 && !wait.warp(g_full, w.round & 1, 7)) alive = false;
+        if (!alive) return;
+        product_nt<T, HD>(tmem + 256, g_tile, v_ring + (t % VR) * TILE, w.columns(w.j));
         commit(dp_full);
-        commit(v_empty(j % VR));
+        if (w.last()) commit(g_empty);
       };
-      bool alive = wait.warp(q_full, 0, 7) && wait.warp(k_full(0), 0, 7);
-      if (alive) {
+      QueryWalk cur(p), nxt = cur;
+      nxt.advance();
+      QueryWalk ahd = nxt;
+      if (nxt.valid()) ahd.advance();
+      scores(cur, 0);
+      alive = alive && wait.warp(v_full(0), 0, 7);
+      if (alive) slopes(cur, 0);
+      if (alive && nxt.valid()) scores(nxt, 1);
+      for (int t = 0; alive && cur.valid(); ++t) {
+        if (!(nxt.valid() ? wait.both(v_full((t + 1) % VR), ((t + 1) / VR) & 1, ds_ready, t & 1, 7) : wait.warp(ds_ready, t & 1, 7))) break;
         tcgen05_fence_after();
-        scores(0);
-        alive = wait.warp(g_full, 0, 7) && wait.warp(v_full(0), 0, 7);
-        if (alive) slopes(0);
+        if (nxt.valid()) slopes(nxt, t + 1);
+        if (!alive) break;
+        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (t & 1) * 128, k_ring + (t % KR) * TILE, 0, cur.columns(cur.j) / 16, cur.j > 0);
+        if (cur.last()) commit(done);
+        if (ahd.valid()) scores(ahd, t + 2);
+        cur = nxt;
+        nxt = ahd;
+        if (ahd.valid()) ahd.advance();
       }
-      if (alive && n > 1) {
-        alive = wait.warp(k_full(1), 0, 7);
-        if (alive) scores(1);
-      }
-      for (int j = 0; j < n && alive; ++j) {
-        if (!wait.warp(ds_ready, j & 1, 7)) break;
-        tcgen05_fence_after();
-        if (j + 1 < n) {
-          if (!wait.warp(v_full((j + 1) % VR), ((j + 1) / VR) & 1, 7)) break;
-          slopes(j + 1);
-        }
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (j & 1) * 128, k_ring + (j % KR) * TILE, 0, columns(j) / 16, j > 0);
-        commit(k_empty(j % KR));
-        if (j + 2 < n) {
-          if (!wait.warp(k_full((j + 2) % KR), ((j + 2) / KR) & 1, 7)) break;
-          scores(j + 2);
-        }
-        if (j + 1 == n) commit(done);
-      }
-      __syncwarp();
     }
   } else {
     registers_up<200>();
     const int half = warp >> 2, thread = threadIdx.x & 127;
-    const int token = item.a + thread / p.packed, head = head0 + thread % p.packed;
-    const bool mine = token < item.length;
-    const int64_t row = (static_cast<int64_t>(item.start) + token) * p.heads + head;
     const float c = p.scale * kLog2e;
-    const float lse = mine ? p.lse[row] : 0.0f, delta = mine ? p.delta[row] : 0.0f;
-    const int last_key = min(token, item.length - 1);
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     bool alive = true;
-    for (int j = 0; j < n; ++j) {
-      const int cols = columns(j) - 64 * half;                   // of this warpgroup's 64: the first `cols`, if any
-      const uint32_t s_addr = tmem + lanes + (j & 1) * 128 + 64 * half, dp_addr = tmem + lanes + 256 + 64 * half;
-      const bool partial = j * KEYS + columns(j) - 1 > item.a;
-      const int limit = last_key - j * KEYS - 64 * half;         // columns above it are not this row's
-      if (!wait.warp(s_full(j & 1), (j >> 1) & 1, 8)) { alive = false; break; }
+    int t = 0;
+    // A unit's dq is stored while the next unit's first exponentials are done: `done` comes 800 cycles after the last dS.
+    T* dst = nullptr;
+    auto store = [&](int round) {
+      if (!wait.warp(done, round & 1, 8)) return false;
       tcgen05_fence_after();
-      float prob[64];
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (32 * g < cols) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (32 * g < cols) {
-#pragma unroll
-          for (int e = 32 * g; e < 32 * g + 32; e += 2) {
-            const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
-            prob[e] = exp2_approx(a.x);
-            prob[e + 1] = exp2_approx(a.y);
-          }
-        }
-      if (!wait.warp(dp_full, j & 1, 8)) { alive = false; break; }
-      tcgen05_fence_after();
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (32 * g < cols) {
-          uint32_t x[32], packed[16];
-          tmem_load_32(dp_addr + 32 * g, x);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 slope = mul2(make_float2(prob[32 * g + e], prob[32 * g + e + 1]),
-                                      add2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(-delta, -delta)));
-            x[e] = __float_as_uint(slope.x);
-            x[e + 1] = __float_as_uint(slope.y);
-          }
-          if (partial) {
-            rare();
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * g + e > limit) x[e] = 0u;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-          tmem_store_16(s_addr + 16 * g, packed);
-        }
-      if (j * KEYS + columns(j) > item.length)                   // rows of K behind the document's end
-        clear_rows<BOXES>(k_ring + (j % KR) * TILE, item.length - j * KEYS, columns(j), threadIdx.x, 256);
-      tmem_store_wait();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
-    }
-    if (alive && wait.warp(done, 0, 8)) {
-      tcgen05_fence_after();
-      T* dst = static_cast<T*>(p.out) + row * p.dim + half * (HD / 2);
 #pragma unroll 1
       for (int g = 0; g < HD / 64; ++g) {
         uint32_t o[32];
         tmem_load_32(tmem + lanes + 384 + half * (HD / 2) + 32 * g, o);
-        if (mine) {
+        if (dst) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint4 v;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+            uint32_t* word = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
             for (int f = 0; f < 4; ++f)
-              w[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]) * p.scale, __uint_as_float(o[8 * e + 2 * f + 1]) * p.scale);
+              word[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]) * p.scale, __uint_as_float(o[8 * e + 2 * f + 1]) * p.scale);
             if (half * (HD / 2) + 32 * g + 8 * e < p.dim) *reinterpret_cast<uint4*>(dst + 32 * g + 8 * e) = v;
           }
         }
       }
+      return true;
+    };
+    auto row_of = [&](const QueryWalk& w) {
+      const int token = w.here.a + thread / p.packed;
+      return token < w.here.length ? (static_cast<int64_t>(w.here.start) + token) * p.heads + w.head0 + thread % p.packed : int64_t(-1);
+    };
+    QueryWalk w(p);
+    int64_t row = row_of(w);
+    float lse = row >= 0 ? p.lse[row] : 0.0f, delta = row >= 0 ? p.delta[row] : 0.0f;
+    while (w.valid() && alive) {
+      const int last_key = min(w.here.a + thread / p.packed, w.here.length - 1);
+      QueryWalk following = w;                                     // its statistics are on their way meanwhile
+      following.next_unit();
+      const int64_t next_row = following.valid() ? row_of(following) : int64_t(-1);
+      const float next_lse = next_row >= 0 ? p.lse[next_row] : 0.0f, next_delta = next_row >= 0 ? p.delta[next_row] : 0.0f;
+      for (int j = 0; j < w.n; ++j, ++t) {
+        const int all_cols = w.columns(j), cols = all_cols - 64 * half;            // of this warpgroup's 64: the first `cols`, if any
+        const uint32_t s_addr = tmem + lanes + (t & 1) * 128 + 64 * half, dp_addr = tmem + lanes + 256 + 64 * half;
+        const bool partial = j * KEYS + all_cols - 1 > w.here.a;
+        const int limit = last_key - j * KEYS - 64 * half;         // columns above it are not this row's
+        if (!wait.warp(s_full(t & 1), (t >> 1) & 1, 8)) { alive = false; break; }
+        tcgen05_fence_after();
+        float prob[64];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (32 * g < cols) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (32 * g < cols) {
+#pragma unroll
+            for (int e = 32 * g; e < 32 * g + 32; e += 2) {
+              const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
+              prob[e] = exp2_approx(a.x);
+              prob[e + 1] = exp2_approx(a.y);
+            }
+          }
+        if (j == 0 && t > 0 && !store(w.round - 1)) { alive = false; break; }
+        if (!wait.warp(dp_full, t & 1, 8)) { alive = false; break; }
+        tcgen05_fence_after();
+        if (threadIdx.x == 0) mbar_arrive(v_empty(t % VR));
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (32 * g < cols) {
+            uint32_t x[32], packed[16];
+            tmem_load_32(dp_addr + 32 * g, x);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 slope = mul2(make_float2(prob[32 * g + e], prob[32 * g + e + 1]),
+                                        add2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(-delta, -delta)));
+              x[e] = __float_as_uint(slope.x);
+              x[e + 1] = __float_as_uint(slope.y);
+            }
+            if (partial) {
+              rare();
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (32 * g + e > limit) x[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+            tmem_store_16(s_addr + 16 * g, packed);
+          }
+        if (j * KEYS + all_cols > w.here.length)                   // rows of K behind the document's end
+          clear_rows<BOXES>(k_ring + (t % KR) * TILE, w.here.length - j * KEYS, all_cols, threadIdx.x, 256);
+        tmem_store_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+      dst = row >= 0 ? static_cast<T*>(p.out) + row * p.dim + half * (HD / 2) : nullptr;
+      w = following;
+      row = next_row;
+      lse = next_lse;
+      delta = next_delta;
     }
+    if (alive && t > 0) store(w.round - 1);
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -1155,19 +1244,33 @@ int fill(AttentionParams& p, const AttentionArgs& a, PlanSection which) {
   return rc;
 }
 
-template <auto Kernel>
-int launch_tc(const char* name, const AttentionParams& p, int64_t blocks, int threads, int smem, cudaStream_t stream) {
-  if (blocks > 0x7fffffff) return fail(CT_ERR_UNSUPPORTED, "%s: %lld blocks", name, (long long)blocks);
+int sm_count() {
+  static std::atomic<int> counts[64];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return 1;
+  int n = counts[device & 63].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n < 1) n = 1;
+    counts[device & 63].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// One persistent CTA per SM, or per unit where there are fewer.
+template <auto Kernel, bool PERSISTENT>
+int launch_tc(const char* name, AttentionParams& p, int64_t units, int threads, int smem, cudaStream_t stream) {
+  if (units > 0x3fffffff) return fail(CT_ERR_UNSUPPORTED, "%s: %lld tiles", name, (long long)units);
   static DynamicSmem allowed;
   const int rc = allowed.set(name, reinterpret_cast<const void*>(Kernel), smem);
   if (rc) return rc;
-  Kernel<<<static_cast<unsigned>(blocks), threads, smem, stream>>>(p);
+  p.units = static_cast<int>(units);
+  Kernel<<<PERSISTENT ? std::min(p.units, sm_count()) : p.units, threads, smem, stream>>>(p);
   count_launch(true);
   return check_launch(name);
 }
 
-template <typename T, int HD> int forward(const AttentionArgs& a, const AttentionParams& p, cudaStream_t stream) {
-  return launch_tc<attention_forward_tc_kernel<T, HD>>("attention_forward_tc_kernel", p, a.count[kPlanForward] * p.head_blocks,
+template <typename T, int HD> int forward(const AttentionArgs& a, AttentionParams& p, cudaStream_t stream) {
+  return launch_tc<attention_forward_tc_kernel<T, HD>, false>("attention_forward_tc_kernel", p, a.count[kPlanForward] * p.head_blocks,
                    kForwardThreads, ForwardShape<HD>::kSmem, stream);
 }
 
@@ -1180,11 +1283,11 @@ template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t 
   p.dk = a.dk;
   p.dv = a.dv;
   p.out = a.dq;
-  rc = launch_tc<attention_query_gradient_tc_kernel<T, HD>>("attention_query_gradient_tc_kernel", p,
+  rc = launch_tc<attention_query_gradient_tc_kernel<T, HD>, true>("attention_query_gradient_tc_kernel", p,
                  a.count[kPlanQuery] * p.head_blocks, kBackwardThreads, QueryShape<HD>::kSmem, stream);
   if (rc) return rc;
   p.items = section(a, kPlanKeys);
-  rc = launch_tc<attention_key_gradient_tc_kernel<T, HD>>("attention_key_gradient_tc_kernel", p, a.count[kPlanKeys] * p.kv_heads,
+  rc = launch_tc<attention_key_gradient_tc_kernel<T, HD>, false>("attention_key_gradient_tc_kernel", p, a.count[kPlanKeys] * p.kv_heads,
                  kBackwardThreads, KeyShape<HD>::kSmem, stream);
   if (rc || !a.count[kPlanReduce]) return rc;
   p.items = section(a, kPlanReduce);
