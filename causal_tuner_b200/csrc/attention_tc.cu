@@ -117,8 +117,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
 }
 
 // Instruction descriptor: fp32 accumulator, both operands T, A K-major, M = 128.
-template <typename T> __device__ __forceinline__ uint32_t operand_desc(bool b_mn, int n) {
-  const uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+template <typename T> __device__ __forceinline__ constexpr uint32_t operand_desc(bool b_mn, int n) {
+  constexpr uint32_t type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
 
@@ -133,10 +133,12 @@ __device__ __forceinline__ PlanRecord uniform(PlanRecord r) { return {uniform(r.
 
 // The MMA warp walks its loops as a whole - with uniform control flow descriptors stay in uniform registers, and a chain
 // of MMAs costs few instructions each - and one elected lane issues. (With one lane in the loop an MMA took 110 cycles to issue.)
-// scores: D[128, n] = A[128, HD] . B[n, HD]^T, both tiles as 128-row boxes of 64 channels
+// scores: D[128, 128] = A[128, HD] . B[128, HD]^T, both tiles as 128-row boxes of 64 channels. Always all 128 columns: with
+// both operands in shared memory an MMA is bound by reading them, and fewer columns take no less time.
 template <typename T, int HD>
-__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, int n) {
-  const uint32_t idesc = operand_desc<T>(false, n), a_lo = desc_low(a, 16), b_lo = desc_low(b, 16);
+__device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr uint32_t idesc = operand_desc<T>(false, 128);
+  const uint32_t a_lo = desc_low(a, 16), b_lo = desc_low(b, 16);
   if (elect_one()) {
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
@@ -146,16 +148,16 @@ __device__ __forceinline__ void product_nt(uint32_t d, uint32_t a, uint32_t b, i
   }
 }
 
-// D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major). K step k (16 rows of B) of A starts at
-// column k / SPAN * STRIDE + k % SPAN * 8; steps [first, last).
-template <typename T, int HD, int SPAN, int STRIDE>
-__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, int first, int last, bool accumulate) {
-  const uint32_t idesc = operand_desc<T>(true, HD), b_lo = desc_low(b, BOX_BYTES);
+// D[128, HD] += A (TMEM) . B, B a 128-row tile read along its rows (MN-major), k steps [FIRST, LAST) of 16 rows. Step k of A
+// starts at column k / SPAN * STRIDE + k % SPAN * 8.
+template <typename T, int HD, int SPAN, int STRIDE, int FIRST, int LAST>
+__device__ __forceinline__ void product_tn(uint32_t d, uint32_t a, uint32_t b, bool accumulate) {
+  constexpr uint32_t idesc = operand_desc<T>(true, HD);
+  const uint32_t b_lo = desc_low(b, BOX_BYTES);
   if (elect_one()) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k >= first && k < last)
-        mma_ts(d, a + k / SPAN * STRIDE + k % SPAN * 8, b_lo + k * (2048 >> 4), desc_high(1024), idesc, accumulate || k > 0);
+    for (int k = FIRST; k < LAST; ++k)
+      mma_ts(d, a + k / SPAN * STRIDE + k % SPAN * 8, b_lo + k * (2048 >> 4), desc_high(1024), idesc, accumulate || k > FIRST);
   }
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
@@ -301,6 +303,34 @@ template <int N> __device__ __forceinline__ void registers_up() { asm volatile("
 template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr uint32_t kOutColumn = 256;       // TMEM: S of the stages at 0 and 128, O at 256 and 384
 
+// Two stages of queries and their positions among the document's keys: stage s holds the tokens from a + s * tile_tokens
+// on and sees the keys [0, end[s]).
+struct ForwardWalk : Walk {
+  int tile_tokens, head_blocks, group, packed;
+  int end0, end1, n0, n1, n, head0, shared;
+  __device__ __forceinline__ ForwardWalk(const AttentionParams& p)
+      : Walk(p.items, p.units, p.head_blocks), tile_tokens(p.tile_tokens), head_blocks(p.head_blocks), group(p.heads / p.kv_heads), packed(p.packed) {
+    open();
+  }
+  __device__ __forceinline__ void open() {
+    head0 = unit % head_blocks * packed;
+    shared = head0 / group;
+    const int first1 = here.a + tile_tokens;
+    end0 = min(here.length, first1);
+    end1 = first1 < here.length ? min(here.length, first1 + tile_tokens) : 0;
+    n0 = (end0 + KEYS - 1) / KEYS;
+    n1 = (end1 + KEYS - 1) / KEYS;
+    n = max(n0, n1);
+  }
+  __device__ __forceinline__ void next_unit() {
+    next();
+    open();
+  }
+  __device__ __forceinline__ int count(int s) const { return s ? n1 : n0; }
+  // whether the stage needs more than the first 64 keys of tile j
+  __device__ __forceinline__ bool both_halves(int s, int j) const { return (s ? end1 : end0) > j * KEYS + 64; }
+};
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kernel(const __grid_constant__ AttentionParams p) {
   using Shape = ForwardShape<HD>;
@@ -311,21 +341,23 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
   const uint32_t q_tile = smem_u32(smem), k_ring = q_tile + 2 * TILE, v_ring = k_ring + RING * TILE;
   const uint32_t bars = v_ring + RING * TILE;
   auto q_full = [&](int s) { return bars + 8u * s; };
-  auto s_full = [&](int s) { return bars + 16u + 8u * s; };
-  auto p_full = [&](int s, int h) { return bars + 32u + 16u * s + 8u * h; };
-  auto half_done = [&](int s) { return bars + 64u + 8u * s; };
-  auto o_full = [&](int s) { return bars + 80u + 8u * s; };
-  auto k_full = [&](int r) { return bars + 96u + 8u * r; };
-  auto k_empty = [&](int r) { return bars + 96u + 8u * (RING + r); };
-  auto v_full = [&](int r) { return bars + 96u + 8u * (2 * RING + r); };
-  auto v_empty = [&](int r) { return bars + 96u + 8u * (3 * RING + r); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 96 + 32 * RING);
+  auto q_empty = [&](int s) { return bars + 16u + 8u * s; };
+  auto s_full = [&](int s) { return bars + 32u + 8u * s; };
+  auto p_full = [&](int s, int h) { return bars + 48u + 16u * s + 8u * h; };
+  auto half_done = [&](int s) { return bars + 80u + 8u * s; };
+  auto o_full = [&](int s) { return bars + 96u + 8u * s; };
+  auto k_full = [&](int r) { return bars + 112u + 8u * r; };
+  auto k_empty = [&](int r) { return bars + 112u + 8u * (RING + r); };
+  auto v_full = [&](int r) { return bars + 112u + 8u * (2 * RING + r); };
+  auto v_empty = [&](int r) { return bars + 112u + 8u * (3 * RING + r); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (2 + 2 * RING) * TILE + 112 + 32 * RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
       mbar_init(s_full(s), 1);
       for (int h = 0; h < 2; ++h) mbar_init(p_full(s, h), 4);
       mbar_init(half_done(s), 1);
@@ -347,101 +379,110 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
   tcgen05_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
   const Waiter wait{abort_flag, p.error_flag};
-
-  const PlanRecord item = uniform(p.items[blockIdx.x / p.head_blocks]);
-  const int head0 = static_cast<int>(blockIdx.x % p.head_blocks) * p.packed;
-  const int shared = head0 / (p.heads / p.kv_heads);
-  // stage s holds the tokens from item.a + s * tile_tokens; keys [0, end[s]) are all it can see
-  const int first1 = item.a + p.tile_tokens;
-  const int end0 = min(item.length, first1);
-  const int end1 = first1 < item.length ? min(item.length, first1 + p.tile_tokens) : 0;
-  const int n0 = (end0 + KEYS - 1) / KEYS, n1 = (end1 + KEYS - 1) / KEYS;
-  const int n = max(n0, n1);
-  // keys of tile j that stage needs, in steps of 32 columns
-  auto columns = [](int end, int j) { return min(KEYS, (end - j * KEYS + 31) & ~31); };
+  // Tiles of keys are counted through all units (t, the first of the current unit): ring slots and phases go by it. A
+  // stage's own phases go by the tiles (and units) that it takes part in.
 
   if (warp >= 8) {
-   registers_down<104>();
-   if (warp == 8) {
-    if (lane == 0) {
-      for (int j = 0; j < n; ++j) {
-        const int r = j % RING;
-        const uint32_t free_parity = ((j / RING) & 1) ^ 1;
-        if (j == 0) {
-          for (int s = 0; s < (n1 ? 2 : 1); ++s) {
+    registers_down<104>();
+    if (warp == 8) {
+      bool alive = true;
+      int t = 0, loads0 = 0, loads1 = 0;
+      for (ForwardWalk w(p); w.valid() && alive; w.next_unit()) {
+        auto load_q = [&](int s, int& loads) {
+          if (!wait.warp(q_empty(s), (loads & 1) ^ 1, 6)) { alive = false; return; }
+          ++loads;
+          if (elect_one()) {
             mbar_expect_tx(q_full(s), TILE);
             for (int b = 0; b < BOXES; ++b)
-              tma_load_3d(q_tile + s * TILE + b * BOX_BYTES, &p.q, q_full(s), 64 * b, head0, item.start + item.a + s * p.tile_tokens);
-            if (s == 0) {
-              mbar_expect_tx(k_full(0), TILE);
-              for (int b = 0; b < BOXES; ++b)
-                tma_load_3d(k_ring + b * BOX_BYTES, &p.k, k_full(0), 64 * b, shared, item.start);
+              tma_load_3d(q_tile + s * TILE + b * BOX_BYTES, &p.q, q_full(s), 64 * b, w.head0, w.here.start + w.here.a + s * w.tile_tokens);
+          }
+        };
+        load_q(0, loads0);
+        for (int j = 0; j < w.n && alive; ++j, ++t) {
+          const int r = t % RING;
+          const uint32_t free_parity = ((t / RING) & 1) ^ 1;
+          if (!wait.warp(k_empty(r), free_parity, 6)) { alive = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(k_full(r), TILE);
+            for (int b = 0; b < BOXES; ++b)
+              tma_load_3d(k_ring + r * TILE + b * BOX_BYTES, &p.k, k_full(r), 64 * b, w.shared, w.here.start + j * KEYS);
+          }
+          if (j == 0 && w.n1) load_q(1, loads1);
+          if (!alive || !wait.warp(v_empty(r), free_parity, 6)) { alive = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(v_full(r), TILE);
+            for (int b = 0; b < BOXES; ++b)
+              tma_load_3d(v_ring + r * TILE + b * BOX_BYTES, &p.v, v_full(r), 64 * b, w.shared, w.here.start + j * KEYS);
+          }
+        }
+      }
+    } else if (warp == 9) {
+      int tiles[2] = {0, 0}, halves[2] = {0, 0}, units[2] = {0, 0};          // per stage
+      auto scores = [&](const ForwardWalk& w, int s, int j, int t) {
+        product_nt<T, HD>(tmem + s * 128, q_tile + s * TILE, k_ring + (t % RING) * TILE);
+        commit(s_full(s));
+        if (j + 1 == w.count(s)) commit(q_empty(s));
+      };
+      ForwardWalk w(p);
+      bool alive = wait.warp(q_full(0), 0, 7) && wait.warp(k_full(0), 0, 7);
+      if (alive) {
+        tcgen05_fence_after();
+        scores(w, 0, 0, 0);
+        ++units[0];
+        if (w.n1) {
+          alive = wait.warp(q_full(1), 0, 7);
+          if (alive) scores(w, 1, 0, 0);
+          ++units[1];
+        }
+        commit(k_empty(0));
+      }
+      for (int t0 = 0; w.valid() && alive;) {
+        ForwardWalk following = w;
+        following.next_unit();
+        for (int j = 0; j < w.n && alive; ++j) {
+          const int t = t0 + j, r = t % RING, next = (t + 1) % RING;
+          const uint32_t next_parity = ((t + 1) / RING) & 1;
+          if (!wait.warp(v_full(r), (t / RING) & 1, 7)) { alive = false; break; }
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int count = w.count(s);
+            if (j < count) {
+              if (!wait.warp(p_full(s, 0), tiles[s] & 1, 7)) { alive = false; break; }
+              tcgen05_fence_after();
+              product_tn<T, HD, 8, 64, 0, 4>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, j > 0);
+              commit(half_done(s));
+              ++tiles[s];
+              if (w.both_halves(s, j)) {
+                if (!wait.warp(p_full(s, 1), halves[s] & 1, 7)) { alive = false; break; }
+                ++halves[s];
+                tcgen05_fence_after();
+                product_tn<T, HD, 8, 64, 4, 8>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, true);
+              }
+              if (j + 1 == count) commit(o_full(s));
+            }
+            if (s == 1) commit(v_empty(r));
+            if (j + 1 < w.n) {
+              if (s == 0 && !wait.warp(k_full(next), next_parity, 7)) { alive = false; break; }
+              if (j + 1 < count) scores(w, s, j + 1, t + 1);
+              if (s == 1) commit(k_empty(next));
+            } else if (following.valid()) {                        // the next unit's first scores
+              if (following.count(s)) {
+                if (!wait.warp(q_full(s), units[s] & 1, 7) || (s == 0 && !wait.warp(k_full(next), next_parity, 7))) { alive = false; break; }
+                ++units[s];
+                scores(following, s, 0, t + 1);
+              }
+              if (s == 1) commit(k_empty(next));
             }
           }
-        } else {
-          if (!wait(k_empty(r), free_parity, 6)) break;
-          mbar_expect_tx(k_full(r), TILE);
-          for (int b = 0; b < BOXES; ++b)
-            tma_load_3d(k_ring + r * TILE + b * BOX_BYTES, &p.k, k_full(r), 64 * b, shared, item.start + j * KEYS);
         }
-        if (!wait(v_empty(r), free_parity, 6)) break;
-        mbar_expect_tx(v_full(r), TILE);
-        for (int b = 0; b < BOXES; ++b)
-          tma_load_3d(v_ring + r * TILE + b * BOX_BYTES, &p.v, v_full(r), 64 * b, shared, item.start + j * KEYS);
+        t0 += w.n;
+        w = following;
       }
     }
-    __syncwarp();
-   } else if (warp == 9) {
-    auto scores = [&](int s, int j) {
-      product_nt<T, HD>(tmem + s * 128, q_tile + s * TILE, k_ring + (j % RING) * TILE, columns(s ? end1 : end0, j));
-      commit(s_full(s));
-    };
-    bool alive = wait.warp(q_full(0), 0, 7) && wait.warp(k_full(0), 0, 7);
-    if (alive) {
-      tcgen05_fence_after();
-      scores(0, 0);
-      if (n1) {
-        alive = wait.warp(q_full(1), 0, 7);
-        if (alive) scores(1, 0);
-      }
-      commit(k_empty(0));
-    }
-    for (int j = 0; j < n && alive; ++j) {
-      const int r = j % RING, next = (j + 1) % RING;
-      if (!wait.warp(v_full(r), (j / RING) & 1, 7)) break;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int count = s ? n1 : n0, end = s ? end1 : end0;
-        if (j < count) {
-          const int steps = columns(end, j) / 16;
-          if (!wait.warp(p_full(s, 0), j & 1, 7)) { alive = false; break; }
-          tcgen05_fence_after();
-          product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, 0, min(steps, 4), j > 0);
-          commit(half_done(s));
-          if (steps > 4) {
-            if (!wait.warp(p_full(s, 1), j & 1, 7)) { alive = false; break; }
-            tcgen05_fence_after();
-            product_tn<T, HD, 8, 64>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, 4, steps, true);
-          }
-          if (j + 1 == count) commit(o_full(s));
-        }
-        if (s == 1) commit(v_empty(r));
-        if (j + 1 < n && s == 0 && !wait.warp(k_full(next), ((j + 1) / RING) & 1, 7)) { alive = false; break; }
-        if (j + 1 < count) scores(s, j + 1);
-        if (s == 1 && j + 1 < n) commit(k_empty(next));
-      }
-    }
-    __syncwarp();
-   }
   } else {
     registers_up<200>();
     const int s = warp >> 2, thread = threadIdx.x & 127;
-    const int count = s ? n1 : n0, end = s ? end1 : end0;
-    const int first = item.a + s * p.tile_tokens;              // the stage's first token
-    const int token = first + thread / p.packed, head = head0 + thread % p.packed;
-    const int last_key = min(token, item.length - 1);
-    const bool negative = p.scale < 0.0f;
-    const float c = fabsf(p.scale) * kLog2e;
+    const float c = p.scale * kLog2e;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;          // this warp's 32 TMEM lanes
     const uint32_t s_addr = tmem + lanes + s * 128, o_addr = tmem + lanes + kOutColumn + s * 128;
     // fp16: probabilities are kept 2^7 above their size (at most 2^15 with the late rescaling), so that small ones do not
@@ -450,35 +491,73 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     float top = -INFINITY, sum = 0.0f;
     bool alive = true;
     const float2 c2 = make_float2(c, c);
-    for (int j = 0; j < count && alive; ++j) {
-      const int cols = columns(end, j);
+    // A unit's output is stored behind the next unit's first exponentials: the last P V is complete by then.
+    bool pending = false;
+    int finished = 0, release_v = -1;
+    int64_t out_row = -1;
+    float out_top = 0.0f, out_sum = 0.0f;
+    auto store = [&]() {
+      if (!wait.warp(o_full(s), finished & 1, 8)) return false;
+      ++finished;
+      pending = false;
+      tcgen05_fence_after();
+      const float factor = 1.0f / out_sum;
+      T* dst = static_cast<T*>(p.out) + out_row * p.dim;
+      if (out_row >= 0 && p.lse) p.lse[out_row] = out_top * c + log2f(out_sum) - kLift;
+#pragma unroll 1
+      for (int g = 0; g < HD / 32; ++g) {
+        uint32_t o[32];
+        tmem_load_32(o_addr + 32 * g, o);
+        if (out_row >= 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 v;
+            uint32_t* word = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              word[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * factor, __uint_as_float(o[8 * i + 2 * e + 1]) * factor);
+            if (32 * g + 8 * i < p.dim) *reinterpret_cast<uint4*>(dst + 32 * g + 8 * i) = v;
+          }
+        }
+      }
+      return true;
+    };
+    // These threads hold a row of scores each, so they walk the units with less state than ForwardWalk.
+    auto read = [&](int round) { return p.items[min(unit_of_round(round), p.units - 1) / p.head_blocks]; };
+    PlanRecord ahead = read(0);
+    int t0 = 0, tiles = 0;
+    for (int round = 0; unit_of_round(round) < p.units && alive; ++round) {
+      const PlanRecord here = uniform(ahead);
+      ahead = read(round + 1);
+      const int first = here.a + s * p.tile_tokens;                // the stage's first token
+      const int end = first < here.length ? min(here.length, first + p.tile_tokens) : 0, count = (end + KEYS - 1) / KEYS;
+      const int token = first + thread / p.packed;
+      const int last_key = min(token, here.length - 1);
+      const bool last_stage = s == (here.a + p.tile_tokens < here.length ? 1 : 0);
+      // idle in this unit: what the unit's other stage waits for must not wait for the next one
+      if (!count && pending && !store()) { alive = false; break; }
+    for (int j = 0; j < count && alive; ++j, ++tiles) {
+      const int cols = end > j * KEYS + 64 ? KEYS : 64, t = t0 + j;      // the halves this tile needs
       const bool partial = j * KEYS + cols - 1 > first;
       const int limit = last_key - j * KEYS;                   // columns above it are not this row's
-      if (!wait.warp(s_full(s), j & 1, 8)) { alive = false; break; }
+      if (!wait.warp(s_full(s), tiles & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
-      if (j * KEYS + cols > item.length) {
+      if (j * KEYS + cols > here.length) {
         // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
-        if (!wait.warp(v_full(j % RING), (j / RING) & 1, 8)) { alive = false; break; }
-        clear_rows<BOXES>(v_ring + (j % RING) * TILE, item.length - j * KEYS, cols, thread, 128);
+        if (!wait.warp(v_full(t % RING), (t / RING) & 1, 8)) { alive = false; break; }
+        clear_rows<BOXES>(v_ring + (t % RING) * TILE, here.length - j * KEYS, cols, thread, 128);
       }
       // Halves of 64 keys: the first half of P V runs under the exponentials of the second. The exponentials do not wait
       // for the half's maximum: they use the maximum so far, and the half is done again with the new one in the rare
       // case that a score is more than 2^8 above it.
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {                            // (rolled: the MMA warp shares the instruction cache)
         if (64 * h >= cols) break;
         uint32_t x[2][32];
 #pragma unroll
         for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 64 * h + 32 * g, x[g]);
 #pragma unroll
         for (int g = 0; g < 2; ++g) tmem_load_wait(x[g]);
-        if (negative) {
-          rare();
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[g][i] ^= 0x80000000u;
-        }
         if (partial) {
           rare();
 #pragma unroll
@@ -489,6 +568,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
         }
         if (j == 0 && h == 0) {                                // key 0 is every row's: a score, not -infinity
           rare();
+          top = -INFINITY;
+          sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < 32; ++i) top = max3(top, __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
         }
@@ -514,7 +595,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
           rare();
           // O holds the products of all halves so far; the last one issued has to be complete
           const bool issued = h == 1 || j > 0;
-          if (h == 1 && !wait.warp(half_done(s), j & 1, 8)) { alive = false; break; }
+          if (h == 1 && !wait.warp(half_done(s), tiles & 1, 8)) { alive = false; break; }
           tcgen05_fence_after();
           const float factor = exp2_approx((top - best) * c);
           top = best;
@@ -535,35 +616,23 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
         sum += part[0].x + part[0].y;
         tmem_store_32(s_addr + 32 * h, packed);
         tmem_store_wait();
+        if (h == 0 && pending && !store()) { alive = false; break; }       // O is free for this unit's products
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(s, h));
       }
     }
-    if (alive && count && wait.warp(o_full(s), 0, 8)) {
-      tcgen05_fence_after();
-      const float factor = 1.0f / sum;
-      const bool mine = token < item.length;
-      const int64_t row = (static_cast<int64_t>(item.start) + token) * p.heads + head;
-      T* dst = static_cast<T*>(p.out) + row * p.dim;
-      if (mine && p.lse) p.lse[row] = top * c + log2f(sum) - kLift;
-#pragma unroll 1
-      for (int g = 0; g < HD / 32; ++g) {
-        uint32_t o[32];
-        tmem_load_32(o_addr + 32 * g, o);
-        if (mine) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 v;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * factor, __uint_as_float(o[8 * i + 2 * e + 1]) * factor);
-            if (32 * g + 8 * i < p.dim) *reinterpret_cast<uint4*>(dst + 32 * g + 8 * i) = v;
-          }
-        }
+      if (alive && count) {
+        pending = true;
+        const int head = unit_of_round(round) % p.head_blocks * p.packed + thread % p.packed;
+        out_row = token < here.length ? (static_cast<int64_t>(here.start) + token) * p.heads + head : int64_t(-1);
+        out_top = top;
+        out_sum = sum;
       }
+      t0 += (min(here.length, here.a + 2 * p.tile_tokens) + KEYS - 1) / KEYS;      // the tiles of both stages
+      if (count) release_v = last_stage ? (t0 - 1) % RING : -1;
     }
+    if (alive && pending) store();
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -712,12 +781,12 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       __syncwarp();
     } else if (warp == 9) {
       auto scores = [&](int r) {                                 // log2 P / c
-        product_nt<T, HD>(tmem, k_tile, q_ring + r * TILE, 128);
+        product_nt<T, HD>(tmem, k_tile, q_ring + r * TILE);
         subtract_stats<T>(tmem, weights, stats + r * Shape::kStats);
         commit(s_full);
       };
       auto slopes = [&](int r) {                                 // dP - delta
-        product_nt<T, HD>(tmem + 128, v_tile, g_ring + r * TILE, 128);
+        product_nt<T, HD>(tmem + 128, v_tile, g_ring + r * TILE);
         subtract_stats<T>(tmem + 128, weights, stats + r * Shape::kStats + Shape::kStatTile);
         commit(dp_full);
         commit(stat_empty(r));
@@ -734,7 +803,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
         const uint32_t next_parity = ((i + 1) / RING) & 1;
         if (!wait.warp(p_ready, i & 1, 7)) break;
         tcgen05_fence_after();
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 256, tmem, g_ring + r * TILE, 0, 8, i > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride, 0, 8>(tmem + 256, tmem, g_ring + r * TILE, i > 0);
         commit(g_empty(r));
         if (i + 1 < count) {
           if (!wait.warp(q_full(next), next_parity, 7) || !wait.warp(stat_full(next), next_parity, 7)) break;
@@ -742,7 +811,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
         }
         if (!wait.warp(ds_ready, i & 1, 7)) break;
         tcgen05_fence_after();
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + 128, q_ring + r * TILE, 0, 8, i > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride, 0, 8>(tmem + 384, tmem + 128, q_ring + r * TILE, i > 0);
         commit(q_empty(r));
         if (i + 1 < count) {
           if (!wait.warp(g_full(next), next_parity, 7)) break;
@@ -952,7 +1021,8 @@ struct QueryWalk : Walk {
     if (++j == n) next_unit();
   }
   __device__ __forceinline__ bool last() const { return j + 1 == n; }
-  __device__ __forceinline__ int columns(int tile) const { return min(KEYS, (end - tile * KEYS + 31) & ~31); }
+  // whether the tile needs more than its first 64 keys
+  __device__ __forceinline__ bool both_halves(int tile) const { return end > tile * KEYS + 64; }
 };
 
 template <typename T, int HD>
@@ -1041,7 +1111,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       auto scores = [&](const QueryWalk& w, int t) {
         alive = (w.j > 0 || wait.warp(q_full, w.round & 1, 7)) && wait.warp(k_full(t % KR), (t / KR) & 1, 7);
         if (!alive) return;
-        product_nt<T, HD>(tmem + (t & 1) * 128, q_tile, k_ring + (t % KR) * TILE, w.columns(w.j));
+        product_nt<T, HD>(tmem + (t & 1) * 128, q_tile, k_ring + (t % KR) * TILE);
         commit(s_full(t & 1));
         if (w.last()) commit(q_empty);
       };
@@ -1049,7 +1119,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       auto slopes = [&](const QueryWalk& w, int t) {
         if (w.j == 0 && !wait.warp(g_full, w.round & 1, 7)) alive = false;
         if (!alive) return;
-        product_nt<T, HD>(tmem + 256, g_tile, v_ring + (t % VR) * TILE, w.columns(w.j));
+        product_nt<T, HD>(tmem + 256, g_tile, v_ring + (t % VR) * TILE);
         commit(dp_full);
         if (w.last()) commit(g_empty);
       };
@@ -1066,7 +1136,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
         tcgen05_fence_after();
         if (nxt.valid()) slopes(nxt, t + 1);
         if (!alive) break;
-        product_tn<T, HD, kHalfSpan, kHalfStride>(tmem + 384, tmem + (t & 1) * 128, k_ring + (t % KR) * TILE, 0, cur.columns(cur.j) / 16, cur.j > 0);
+        product_tn<T, HD, kHalfSpan, kHalfStride, 0, 4>(tmem + 384, tmem + (t & 1) * 128, k_ring + (t % KR) * TILE, cur.j > 0);
+        if (cur.both_halves(cur.j)) product_tn<T, HD, kHalfSpan, kHalfStride, 4, 8>(tmem + 384, tmem + (t & 1) * 128, k_ring + (t % KR) * TILE, true);
         if (cur.last()) commit(done);
         if (ahd.valid()) scores(ahd, t + 2);
         cur = nxt;
@@ -1118,36 +1189,33 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       const int64_t next_row = following.valid() ? row_of(following) : int64_t(-1);
       const float next_lse = next_row >= 0 ? p.lse[next_row] : 0.0f, next_delta = next_row >= 0 ? p.delta[next_row] : 0.0f;
       for (int j = 0; j < w.n; ++j, ++t) {
-        const int all_cols = w.columns(j), cols = all_cols - 64 * half;            // of this warpgroup's 64: the first `cols`, if any
+        const int all_cols = w.both_halves(j) ? KEYS : 64;
+        const bool idle = half && all_cols == 64;                  // nothing in this warpgroup's 64 columns
         const uint32_t s_addr = tmem + lanes + (t & 1) * 128 + 64 * half, dp_addr = tmem + lanes + 256 + 64 * half;
         const bool partial = j * KEYS + all_cols - 1 > w.here.a;
         const int limit = last_key - j * KEYS - 64 * half;         // columns above it are not this row's
         if (!wait.warp(s_full(t & 1), (t >> 1) & 1, 8)) { alive = false; break; }
         tcgen05_fence_after();
         float prob[64];
+        if (!idle) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (32 * g < cols) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+          for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (32 * g < cols) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
+          for (int g = 0; g < 2; ++g) tmem_load_wait(*reinterpret_cast<uint32_t(*)[32]>(&prob[32 * g]));
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (32 * g < cols) {
-#pragma unroll
-            for (int e = 32 * g; e < 32 * g + 32; e += 2) {
-              const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
-              prob[e] = exp2_approx(a.x);
-              prob[e + 1] = exp2_approx(a.y);
-            }
+          for (int e = 0; e < 64; e += 2) {
+            const float2 a = fma2(make_float2(prob[e], prob[e + 1]), make_float2(c, c), make_float2(-lse, -lse));
+            prob[e] = exp2_approx(a.x);
+            prob[e + 1] = exp2_approx(a.y);
           }
+        }
         if (j == 0 && t > 0 && !store(w.round - 1)) { alive = false; break; }
         if (!wait.warp(dp_full, t & 1, 8)) { alive = false; break; }
         tcgen05_fence_after();
         if (threadIdx.x == 0) mbar_arrive(v_empty(t % VR));
+        if (!idle) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-          if (32 * g < cols) {
+          for (int g = 0; g < 2; ++g) {
             uint32_t x[32], packed[16];
             tmem_load_32(dp_addr + 32 * g, x);
 #pragma unroll
@@ -1167,6 +1235,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
             for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
             tmem_store_16(s_addr + 16 * g, packed);
           }
+        }
         if (j * KEYS + all_cols > w.here.length)                   // rows of K behind the document's end
           clear_rows<BOXES>(k_ring + (t % KR) * TILE, w.here.length - j * KEYS, all_cols, threadIdx.x, 256);
         tmem_store_wait();
@@ -1270,7 +1339,7 @@ int launch_tc(const char* name, AttentionParams& p, int64_t units, int threads, 
 }
 
 template <typename T, int HD> int forward(const AttentionArgs& a, AttentionParams& p, cudaStream_t stream) {
-  return launch_tc<attention_forward_tc_kernel<T, HD>, false>("attention_forward_tc_kernel", p, a.count[kPlanForward] * p.head_blocks,
+  return launch_tc<attention_forward_tc_kernel<T, HD>, true>("attention_forward_tc_kernel", p, a.count[kPlanForward] * p.head_blocks,
                    kForwardThreads, ForwardShape<HD>::kSmem, stream);
 }
 
@@ -1300,9 +1369,9 @@ template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t 
 
 }  // namespace
 
-// The backward pass divides the log-sums by the scale (Split): a scale that would take them out of range goes to the
-// shape-generic kernels.
-bool scale_ok(const AttentionArgs& a) { return std::fabs(a.scale) >= (a.dtype == CT_F16 ? 1e-6f : 1e-20f); }
+// The forward pass takes row maxima of unscaled scores, so the scale has to be positive, and the backward pass divides the
+// log-sums by it (Split), so it must not be tiny; other scales go to the shape-generic kernels.
+bool scale_ok(const AttentionArgs& a) { return a.scale >= (a.dtype == CT_F16 ? 1e-6f : 1e-20f); }
 
 bool attention_tc_supported(const AttentionArgs& a) {
   return scale_ok(a) && (a.dtype == CT_BF16 || a.dtype == CT_F16) && a.head_dim % 8 == 0 && a.head_dim <= 128 && view_ok(a.q) && view_ok(a.k) &&
