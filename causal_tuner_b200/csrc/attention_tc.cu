@@ -789,7 +789,6 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
         product_nt<T, HD>(tmem + 128, v_tile, g_ring + r * TILE);
         subtract_stats<T>(tmem + 128, weights, stats + r * Shape::kStats + Shape::kStatTile);
         commit(dp_full);
-        commit(stat_empty(r));
       };
       bool alive = wait.warp(kv_full, 0, 7) && wait.warp(q_full(0), 0, 7) && wait.warp(stat_full(0), 0, 7);
       if (alive) {
@@ -806,7 +805,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
         product_tn<T, HD, kHalfSpan, kHalfStride, 0, 8>(tmem + 256, tmem, g_ring + r * TILE, i > 0);
         commit(g_empty(r));
         if (i + 1 < count) {
-          if (!wait.warp(q_full(next), next_parity, 7) || !wait.warp(stat_full(next), next_parity, 7)) break;
+          if (!wait.both(q_full(next), next_parity, stat_full(next), next_parity, 7)) break;
           scores(next);
         }
         if (!wait.warp(ds_ready, i & 1, 7)) break;
@@ -854,9 +853,11 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;
     const uint32_t s_addr = tmem + lanes + 64 * half, dp_addr = s_addr + 128;
     bool alive = true;
+    int token0 = tile_token(0) - p.tile_tokens;
     for (int i = 0; i < count; ++i) {
       const int r = i % RING;
-      const int token0 = tile_token(i);
+      token0 += p.tile_tokens;
+      if (token0 >= item.length) token0 = key0;
       // this thread's columns [low, high) of the tile: queries at or after its key, inside the document
       const bool partial = token0 < key0 + 127 || token0 + p.tile_tokens > item.length;
       const int low = (key - token0) * p.packed - 64 * half, high = (item.length - token0) * p.packed - 64 * half;
@@ -901,6 +902,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       if (lane == 0) mbar_arrive(p_ready);
       if (!wait.warp(dp_full, i & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
+      if (threadIdx.x == 0) mbar_arrive(stat_empty(r));
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         uint32_t x[32], packed[16];
