@@ -360,6 +360,8 @@ __global__ void attention_sum_heads_kernel(const PlanRecord* tiles, AttentionArg
 // lanes with 16 bytes each (VECTOR: rows are whole numbers of 16-byte pieces), or by a warp, element by element.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) attention_delta_kernel(const T* dy, const T* y, float* delta, int64_t rows, int dim, int lanes) {
+  // (inside the query-gradient kernel, by its two idle warps, this cost more than the 48 us of its own at 16384 x 32 rows:
+  // 409 against 281 us for the packed 7B batch)
   constexpr int N = 16 / sizeof(T);
   const int64_t thread = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t row = thread / lanes;

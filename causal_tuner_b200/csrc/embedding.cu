@@ -16,7 +16,10 @@ namespace {
 
 constexpr int kRadixBits = 8, kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kBlockItems = 4 * kSortThreads;          // sorted by one block of the many-block sort
+// Tokens per thread of the many-block sort: one, so that 16384 tokens are 16 blocks, four where the blocks' histograms
+// (which every block sums) would otherwise weigh more than the tokens.
+constexpr int kManySteps = 4;
+constexpr int64_t kOneStepTokens = 65536;
 constexpr int kOneBlockItems = 4 * kSortThreads;       // up to here one block sorts alone, in shared memory, in one launch
 constexpr int kPiece = 32;                             // sorted tokens per piece of a long run
 constexpr int kBadToken = 9;                           // device error code
@@ -203,13 +206,13 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_block_kernel(
   }
 }
 
-constexpr int kBlockSteps = kBlockItems / kSortThreads;
 // The first pass takes its keys from the ids (src_keys null).
-__device__ __forceinline__ void load_items(int (&key)[kBlockSteps], int (&position)[kBlockSteps], const int64_t* ids, const int* src_keys,
+template <int STEPS>
+__device__ __forceinline__ void load_items(int (&key)[STEPS], int (&position)[STEPS], const int64_t* ids, const int* src_keys,
                                            const int* src_positions, int64_t tokens, int64_t rows, int64_t padding, int* error_flag) {
 #pragma unroll
-  for (int k = 0; k < kBlockSteps; ++k) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBlockItems + item_index(k, kBlockItems / kSortWarps);
+  for (int k = 0; k < STEPS; ++k) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * STEPS * kSortThreads + item_index(k, 32 * STEPS);
     key[k] = -1;
     position[k] = 0;
     if (at < tokens) {
@@ -219,26 +222,28 @@ __device__ __forceinline__ void load_items(int (&key)[kBlockSteps], int (&positi
   }
 }
 
+template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_count_kernel(const int64_t* ids, const int* src_keys, int64_t tokens, int64_t rows,
                                                                             int64_t padding, int shift, int* histogram, int* error_flag) {
   __shared__ SortShared s;
-  int key[kBlockSteps], position[kBlockSteps], digit[kBlockSteps];
+  int key[STEPS], position[STEPS], digit[STEPS];
   load_items(key, position, ids, src_keys, src_keys, tokens, rows, padding, error_flag);
 #pragma unroll
-  for (int k = 0; k < kBlockSteps; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
+  for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
   count_digits(s, digit);
   const int total = sum_over_warps(s);
   if (threadIdx.x < kRadix) histogram[static_cast<int64_t>(blockIdx.x) * kRadix + threadIdx.x] = total;
 }
 
+template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(const int64_t* ids, const int* src_keys, const int* src_positions,
                                                                               int64_t tokens, int64_t rows, int64_t padding, int shift,
                                                                               const int* histogram, int* keys, int* positions, int* error_flag) {
   __shared__ SortShared s;
-  int key[kBlockSteps], position[kBlockSteps], digit[kBlockSteps];
+  int key[STEPS], position[STEPS], digit[STEPS];
   load_items(key, position, ids, src_keys, src_positions, tokens, rows, padding, error_flag);
 #pragma unroll
-  for (int k = 0; k < kBlockSteps; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
+  for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
   count_digits(s, digit);
   sum_over_warps(s);
   // every block sums the histogram for itself: the digit's items in all blocks, and in the blocks before this one
@@ -393,7 +398,8 @@ __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a)
 bool known(int dtype) { return dtype == CT_F32 || dtype == CT_BF16 || dtype == CT_F16; }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-int64_t sort_blocks(int64_t tokens) { return (tokens + kBlockItems - 1) / kBlockItems; }
+int sort_steps(int64_t tokens) { return tokens <= kOneStepTokens ? 1 : kManySteps; }
+int64_t sort_blocks(int64_t tokens) { return (tokens + sort_steps(tokens) * kSortThreads - 1) / (sort_steps(tokens) * kSortThreads); }
 int64_t piece_count(int64_t tokens) { return (tokens + kPiece - 1) / kPiece; }
 
 template <typename F> int by_type(int dtype, F f) {
@@ -432,9 +438,10 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
     int* to_keys = last_is_first ? keys : other_keys;
     int* to_positions = last_is_first ? positions : other_positions;
     const int shift = pass * kRadixBits;
-    embedding_sort_count_kernel<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
-    embedding_sort_scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, from_positions, tokens, rows, padding, shift, histogram,
-                                                                       to_keys, to_positions, error_flag);
+    const auto count = sort_steps(tokens) == 1 ? embedding_sort_count_kernel<1> : embedding_sort_count_kernel<kManySteps>;
+    const auto scatter = sort_steps(tokens) == 1 ? embedding_sort_scatter_kernel<1> : embedding_sort_scatter_kernel<kManySteps>;
+    count<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
+    scatter<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, from_positions, tokens, rows, padding, shift, histogram, to_keys, to_positions, error_flag);
     for (int i = 0; i < 2; ++i) count_launch(false);
     from_keys = to_keys;
     from_positions = to_positions;
@@ -503,7 +510,7 @@ extern "C" int ct_embedding_gradient(const void* dy, int64_t ld, const int64_t* 
   if (!known(dy_dtype) || !known(table_dtype)) return fail(CT_ERR_ARG, "ct_embedding_gradient: dtype");
   if (rows == 0 || width == 0) return CT_OK;
   if (!d_table || !workspace || (tokens > 0 && (!dy || !ids))) return fail(CT_ERR_ARG, "ct_embedding_gradient: null pointer");
-  if (tokens >= (int64_t(1) << 31) - kBlockItems || rows >= (int64_t(1) << 31) - 1024)
+  if (tokens >= (int64_t(1) << 31) - 65536 || rows >= (int64_t(1) << 31) - 1024)
     return fail(CT_ERR_UNSUPPORTED, "ct_embedding_gradient: %lld tokens, %lld rows", (long long)tokens, (long long)rows);
   int* flag = device_error_flag();
   if (!flag) return fail(CT_ERR_CUDA, "cannot allocate the device error flag");

@@ -1,6 +1,7 @@
 """Document attention (kernels/attention_cuda.py) against 64-bit values with derived bounds."""
 
 import random
+import threading
 
 import pytest
 import torch
@@ -256,6 +257,25 @@ def test_on_another_stream_and_in_a_graph(dtype):
             graph.replay()
         for graph, outputs in graphs:
             assert all(torch.equal(a, b) for a, b in zip(outputs, results.values()))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_from_a_thread_that_has_not_used_cuda(dtype):
+    spans = documents(1, 200, 4, 150)
+    q, k, v, dy = tensors(1, 200, 4, 1, 64, dtype)
+    plan = prepare_documents((1, 200), spans, "cuda", 4)
+    y, lse = attention_forward(q, k, v, plan)
+    expected = (y, *attention_backward(dy, q, k, v, y, lse, plan))
+    torch.cuda.synchronize()
+    results = {}
+    forward = threading.Thread(target=lambda: results.update(forward=attention_forward(q, k, v, plan)))
+    backward = threading.Thread(target=lambda: results.update(backward=attention_backward(dy, q, k, v, y, lse, plan)))
+    for thread in (forward, backward):
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(results["forward"][0], y) and torch.equal(results["forward"][1], lse)
+    assert all(torch.equal(a, b) for a, b in zip(results["backward"], expected[1:]))
 
 
 def test_refusals():
