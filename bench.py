@@ -406,7 +406,7 @@ def finish(args, rank, world_size, distributed, ms_per_step, e2e_ms, e2e_steps, 
 STEP_METRIC = "train tokens/s (NF4 r256 LoRA, MQA decoder, one optimizer update)"
 
 
-def step_config(name, gpus, mlp_cache_gib=0, execution=None, keep_low_rank=False):
+def step_config(name, gpus, mlp_cache_gib=0, execution=None, keep_low_rank=False, attention="flash_attention_2"):
     import bench_step
     spec = bench_step.WORKLOADS[name]
     config = spec["config"]
@@ -416,7 +416,9 @@ def step_config(name, gpus, mlp_cache_gib=0, execution=None, keep_low_rank=False
     kept_mb = 5 * bench_step.RANK * 2 * spec["rows"] * spec["length"] / 1e6
     return {"workload": f"{name} ({spec['reference']})", **spec["config"], "rank": bench_step.RANK,
             "rows_per_gpu": spec["rows"], "seq_len": spec["length"], "global_batch": spec["rows"] * gpus,
-            "nf4_blocksize": 64, "absmax": "fp32", "attention": "flash_attention_2 (library, as in the reference)",
+            "nf4_blocksize": 64, "absmax": "fp32",
+            "attention": ("flash_attention_2 (library, as in the reference)" if attention == "flash_attention_2"
+                          else "documents (this package's kernels)"),
             "activation_checkpointing": False,
             "mlp": (f"gate/up kept for backward in {cached} layers ({mlp_cache_gib} GiB budget, last layers first), "
                     f"recomputed in backward in the others"),
@@ -718,7 +720,8 @@ def run_step(args):
     if args.layers:        # profiler-sized case: fewer layers of the same shapes (not a bench value)
         spec = dict(spec, config=dict(spec["config"], num_hidden_layers=args.layers))
         bench_step.WORKLOADS[args.workload] = spec
-    model = bench_step.build_model(args.workload, device, args.mlp_cache_gib, keep_low_rank=bool(args.keep_low_rank))
+    model = bench_step.build_model(args.workload, device, args.mlp_cache_gib, keep_low_rank=bool(args.keep_low_rank),
+                                   attention=args.attention)
     optimizer = make_optimizer(model, learning_rate=2e-5)
     trainer = Trainer(model, optimizer, device=device, loss_token_budget=4096)
     # One global batch of world_size x rows packed rows, the same on every rank; each rank takes the rows
@@ -817,7 +820,7 @@ def run_step(args):
         "steps": args.steps, "warmup": max(args.warmup, 3), "ms_per_step": ms_per_step, "higher_is_better": True,
         "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
         "config": step_config(args.workload, world_size, args.mlp_cache_gib, model.last_execution,
-                              bool(args.keep_low_rank)),
+                              bool(args.keep_low_rank), args.attention),
         "step_tflops_per_gpu": flops / (ms_per_step * 1e-3) / 1e12,
         "step_frac_of_bf16_peak": flops / (ms_per_step * 1e-3) / 1e12 / peak,
         "e2e": {"value": tokens / (e2e_ms * 1e-3), "unit": "tokens/s", "h2d_bytes_per_step": h2d,
@@ -861,6 +864,9 @@ def main():
     parser.add_argument("--mlp-cache-gib", type=float, default=64.0,
                         help="per-GPU byte budget for keeping MLP gate/up activations instead of recomputing them "
                              "(0: always recompute)")
+    parser.add_argument("--attention", choices=("flash_attention_2", "documents"), default="flash_attention_2",
+                        help="attention of the step workloads: the library's kernels, as the reference calls them, or "
+                             "this package's document attention (kernels/attention_cuda.py)")
     parser.add_argument("--workload", choices=("step7b", "step1b", "projection", "shapes"), default="step7b",
                         help="step7b: 7B-class decoder update (the headline metric); step1b: the 1.3B decoder; "
                              "projection: one fused NF4+LoRA projection, forward+backward; shapes: the GEMM shapes of a "

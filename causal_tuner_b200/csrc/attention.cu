@@ -467,7 +467,7 @@ int describe(AttentionArgs& a, const char* name, const int32_t* plan, const int6
     return fail(CT_ERR_ARG, "%s: sizes (tokens %lld, heads %d, kv_heads %d, head_dim %d)", name, (long long)tokens, heads, kv_heads, head_dim);
   if (!known(dtype)) return fail(CT_ERR_ARG, "%s: dtype", name);
   if (head_dim > 128) return fail(CT_ERR_UNSUPPORTED, "%s: head_dim %d is above 128", name, head_dim);
-  if (heads > 65535) return fail(CT_ERR_UNSUPPORTED, "%s: %d heads", name, heads);
+  if (heads > 65535 || kv_heads > 32767) return fail(CT_ERR_UNSUPPORTED, "%s: %d heads, %d key heads", name, heads, kv_heads);
   if (tokens >= (int64_t(1) << 31) - 256) return fail(CT_ERR_UNSUPPORTED, "%s: %lld tokens", name, (long long)tokens);
   if (!sections) return fail(CT_ERR_ARG, "%s: null sections", name);
   a = AttentionArgs{};

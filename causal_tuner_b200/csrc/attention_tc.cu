@@ -860,7 +860,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
       if (token0 >= item.length) token0 = key0;
       // this thread's columns [low, high) of the tile: queries at or after its key, inside the document
       const bool partial = token0 < key0 + 127 || token0 + p.tile_tokens > item.length;
-      const int low = (key - token0) * p.packed - 64 * half, high = (item.length - token0) * p.packed - 64 * half;
+      // (clamped to the tile, so that the products fit for documents of any length)
+      const int low = max(key - token0, 0) * p.packed - 64 * half, high = min(item.length - token0, p.tile_tokens) * p.packed - 64 * half;
       if (!wait.warp(s_full, i & 1, 8)) { alive = false; break; }
       tcgen05_fence_after();
       float prob[64];
@@ -1368,7 +1369,6 @@ template <typename T, int HD> int backward(const AttentionArgs& a, cudaStream_t 
                  kBackwardThreads, KeyShape<HD>::kSmem, stream);
   if (rc || !a.count[kPlanReduce]) return rc;
   p.items = section(a, kPlanReduce);
-  if (a.kv_heads > 32767) return fail(CT_ERR_UNSUPPORTED, "ct_attention_backward: %d key heads", a.kv_heads);
   const dim3 grid(a.count[kPlanReduce], (128 * a.head_dim / 4 + 255) / 256, 2 * a.kv_heads);
   attention_sum_pieces_kernel<T><<<grid, 256, 0, stream>>>(p);
   count_launch(false);

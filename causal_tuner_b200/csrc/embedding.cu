@@ -57,6 +57,7 @@ template <typename W, typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const int64_t* ids, const W* table, T* out, int64_t tokens,
                                                                 int64_t rows, int64_t width, float scale, int* error_flag) {
   const int64_t per_row = VECTOR ? width / 8 : width, total = tokens * per_row;
+#pragma unroll 1
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t token = i / per_row, column = (i - token * per_row) * (VECTOR ? 8 : 1);
     const int64_t id = ids[token];

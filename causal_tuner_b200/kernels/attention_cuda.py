@@ -36,6 +36,7 @@ class DocumentPlan:
     sections: tuple                 # ((first record, count), ...) of the six sections
     key_slots: int
     host_sections: ctypes.Array = field(repr=False, compare=False, default=None)
+    stream: int = 0                 # raw handle of the stream on which the table was made
 
 
 def _tiles(starts, lengths, step):
@@ -79,7 +80,8 @@ def _key_sections(starts, lengths, tile_tokens, head_blocks, kv_heads):
 
 def prepare_documents(shape, spans, device, heads, kv_heads=1):
     """The plan of a [rows, width] batch whose documents are `spans`, ((row, start, end), ...) as `segments.runs` gives
-    them: any order, gaps allowed, no token in two documents."""
+    them: any order, gaps allowed, no token in two documents. A captured graph reads the plan's table when it is replayed:
+    keep the plan as long as the graph."""
     rows, width = (int(n) for n in shape)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
@@ -112,7 +114,18 @@ def prepare_documents(shape, spans, device, heads, kv_heads=1):
     sections = tuple((int(first[i]), len(part) // 2 if i == 2 else len(part)) for i, part in enumerate(parts))
     records = numpy.ascontiguousarray(numpy.concatenate(parts), dtype=numpy.int32)
     host = (ctypes.c_int64 * 12)(*(n for pair in sections for n in pair))
-    return DocumentPlan((rows, width), heads, kv_heads, spans, torch.from_numpy(records).to(device), sections, slots, host)
+    table = torch.from_numpy(records).to(device)
+    return DocumentPlan((rows, width), heads, kv_heads, spans, table, sections, slots, host,
+                        _lib.stream_of(table) if table.is_cuda else 0)
+
+
+def _stream(plan, tensor):
+    """The stream to launch on. A plan may be dropped as soon as the host has issued the calls that read it: where that is
+    another stream than the table's own, the allocator is told."""
+    stream = _lib.stream_of(tensor)
+    if stream != plan.stream and not torch.cuda.is_current_stream_capturing():
+        plan.table.record_stream(torch.cuda.current_stream(tensor.device))
+    return stream
 
 
 def _check(q, k, v, plan):
@@ -174,7 +187,7 @@ def attention_forward(q, k, v, plan, *, scale=None, keep_lse=True):
         path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
         _lib.check(library.ct_attention_forward(
             *operands, out.data_ptr(), _lib.pointer(lse), plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads,
-            dim, scale, code, path, _lib.stream_of(q)))
+            dim, scale, code, path, _stream(plan, q)))
     return out, lse
 
 
@@ -209,7 +222,7 @@ def attention_backward(dy, q, k, v, y, lse, plan, *, scale=None):
         _lib.check(library.ct_attention_backward(
             *operands, y.data_ptr(), lse.data_ptr(), dy.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads, dim, scale, code, path, workspace.data_ptr(),
-            _lib.stream_of(q)))
+            _stream(plan, q)))
     return dq, dk, dv
 
 

@@ -70,6 +70,15 @@ def test_heads_and_types(dtype, heads, kv_heads, dim):
     check(*tensors(2, 301, heads, kv_heads, dim, dtype), spans)
 
 
+@pytest.mark.parametrize("dtype, dim", [("bf16", 128), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("heads, kv_heads", [(32, 1), (16, 16), (12, 4), (40, 8)])
+@pytest.mark.parametrize("longest, gap", [(30, 0), (300, 17), (1400, 3)])
+def test_more_tiles_than_the_gpu_has_sms(dtype, dim, heads, kv_heads, longest, gap):
+    """Several tiles of queries, of unequal length, per persistent block; short documents leave its second stage empty."""
+    spans = documents(3, 1400, 21, longest, gap=gap)
+    check(*tensors(3, 1400, heads, kv_heads, dim, dtype), spans)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 385, 700])
 @pytest.mark.parametrize("heads, kv_heads", [(2, 2), (4, 1)])
@@ -257,6 +266,25 @@ def test_on_another_stream_and_in_a_graph(dtype):
             graph.replay()
         for graph, outputs in graphs:
             assert all(torch.equal(a, b) for a, b in zip(outputs, results.values()))
+
+
+def test_a_plan_may_be_dropped_once_the_calls_are_issued():
+    spans = documents(2, 700, 4, 300, gap=3)
+    q, k, v, dy = tensors(2, 700, 8, 1, 64, "bf16")
+    expected = run(q, k, v, dy, spans)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    for _ in range(20):
+        plan = prepare_documents((2, 700), spans, "cuda", 8)
+        torch.cuda.current_stream().synchronize()
+        with torch.cuda.stream(stream):
+            y, lse = attention_forward(q, k, v, plan)
+            grads = attention_backward(dy, q, k, v, y, lse, plan)
+        records = plan.table.numel()
+        del plan
+        torch.full((records,), 7, device="cuda", dtype=torch.int32)       # where the table was, if it were given away
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((y, *grads), expected.values()))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
