@@ -57,8 +57,8 @@ template <typename W, typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const int64_t* ids, const W* table, T* out, int64_t tokens,
                                                                 int64_t rows, int64_t width, float scale, int* error_flag) {
   const int64_t per_row = VECTOR ? width / 8 : width, total = tokens * per_row;
-#pragma unroll 1
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += step) {
     const int64_t token = i / per_row, column = (i - token * per_row) * (VECTOR ? 8 : 1);
     const int64_t id = ids[token];
     const bool known = id >= 0 && id < rows;
@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const int64_t* i
 }
 
 // ---- stable radix sort of (key, position) --------------------------------------------------
-// A block ranks its items by one digit: every warp owns a contiguous stretch, counts its digits, the counts are summed over
-// digits and warps, and the warp goes over its stretch again handing out places in order.
+// A block ranks its items by one digit: every warp owns a contiguous stretch and counts its digits in order, which gives each
+// item its rank; the counts are summed over warps and digits, and every item goes to its place.
 struct SortShared {
   int counts[kSortWarps][kRadix];
   int digit_base[kRadix];
@@ -95,13 +95,16 @@ __device__ __forceinline__ uint32_t same_digit(int digit) {
   return peers;
 }
 
-template <int STEPS> __device__ __forceinline__ void count_digits(SortShared& s, const int (&digit)[STEPS]) {
+// Counts the warp's digits; rank[k] = items of the same digit before item k in the warp's stretch.
+template <int STEPS> __device__ __forceinline__ void count_digits(SortShared& s, const int (&digit)[STEPS], int (&rank)[STEPS]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = lane; i < kRadix; i += 32) s.counts[warp][i] = 0;
   __syncwarp();
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     const uint32_t peers = same_digit(digit[k]);
+    rank[k] = digit[k] >= 0 ? s.counts[warp][digit[k]] + __popc(peers & ((1u << lane) - 1)) : 0;
+    __syncwarp();
     if (digit[k] >= 0 && lane == __ffs(peers) - 1) s.counts[warp][digit[k]] += __popc(peers);
     __syncwarp();
   }
@@ -143,18 +146,12 @@ __device__ __forceinline__ void digit_sums(SortShared& s, int value) {
   __syncthreads();
 }
 
-template <int STEPS, typename Place> __device__ __forceinline__ void hand_out(SortShared& s, const int (&digit)[STEPS], Place place) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+template <int STEPS, typename Place>
+__device__ __forceinline__ void hand_out(const SortShared& s, const int (&digit)[STEPS], const int (&rank)[STEPS], Place place) {
+  const int warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int k = 0; k < STEPS; ++k) {
-    const uint32_t peers = same_digit(digit[k]);
-    int at = 0;
-    if (digit[k] >= 0) at = s.digit_base[digit[k]] + s.counts[warp][digit[k]] + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (digit[k] >= 0 && lane == __ffs(peers) - 1) s.counts[warp][digit[k]] += __popc(peers);
-    __syncwarp();
-    if (digit[k] >= 0) place(k, at);
-  }
+  for (int k = 0; k < STEPS; ++k)
+    if (digit[k] >= 0) place(k, s.digit_base[digit[k]] + s.counts[warp][digit[k]] + rank[k]);
 }
 
 // Tokens of the padding row and of ids outside the table get the key `rows`: behind every row's run.
@@ -173,10 +170,11 @@ __device__ __forceinline__ int item_index(int k, int items_per_warp) {
 template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_block_kernel(const int64_t* ids, int tokens, int64_t rows, int64_t padding,
                                                                                 int bits, int* keys, int* positions, int* error_flag) {
+  grid_dependency_wait();
   extern __shared__ int2 items[];                       // (key, position)
   __shared__ SortShared s;
   int2 mine[STEPS];
-  int digit[STEPS];
+  int digit[STEPS], rank[STEPS];
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     const int at = item_index(k, 32 * STEPS);
@@ -185,10 +183,10 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_block_kernel(
   for (int shift = 0; shift < bits; shift += kRadixBits) {
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) digit[k] = mine[k].x < 0 ? -1 : (mine[k].x >> shift) & (kRadix - 1);
-    count_digits(s, digit);
+    count_digits(s, digit, rank);
     const int total = sum_over_warps(s);
     digit_sums(s, total);
-    hand_out(s, digit, [&](int k, int at) { items[at] = mine[k]; });
+    hand_out(s, digit, rank, [&](int k, int at) { items[at] = mine[k]; });
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) {
@@ -226,12 +224,13 @@ __device__ __forceinline__ void load_items(int (&key)[STEPS], int (&position)[ST
 template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_count_kernel(const int64_t* ids, const int* src_keys, int64_t tokens, int64_t rows,
                                                                             int64_t padding, int shift, int* histogram, int* error_flag) {
+  grid_dependency_wait();
   __shared__ SortShared s;
-  int key[STEPS], position[STEPS], digit[STEPS];
+  int key[STEPS], position[STEPS], digit[STEPS], rank[STEPS];
   load_items(key, position, ids, src_keys, src_keys, tokens, rows, padding, error_flag);
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
-  count_digits(s, digit);
+  count_digits(s, digit, rank);
   const int total = sum_over_warps(s);
   if (threadIdx.x < kRadix) histogram[static_cast<int64_t>(blockIdx.x) * kRadix + threadIdx.x] = total;
 }
@@ -240,12 +239,13 @@ template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(const int64_t* ids, const int* src_keys, const int* src_positions,
                                                                               int64_t tokens, int64_t rows, int64_t padding, int shift,
                                                                               const int* histogram, int* keys, int* positions, int* error_flag) {
+  grid_dependency_wait();
   __shared__ SortShared s;
-  int key[STEPS], position[STEPS], digit[STEPS];
+  int key[STEPS], position[STEPS], digit[STEPS], rank[STEPS];
   load_items(key, position, ids, src_keys, src_positions, tokens, rows, padding, error_flag);
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
-  count_digits(s, digit);
+  count_digits(s, digit, rank);
   sum_over_warps(s);
   // every block sums the histogram for itself: the digit's items in all blocks, and in the blocks before this one
   int total = 0, before = 0;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(co
   digit_sums(s, total);
   if (threadIdx.x < kRadix) s.digit_base[threadIdx.x] += before;
   __syncthreads();
-  hand_out(s, digit, [&](int k, int at) {
+  hand_out(s, digit, rank, [&](int k, int at) {
     keys[at] = key[k];
     positions[at] = position[k];
   });
@@ -275,6 +275,11 @@ struct GradientArgs {
   float* pieces;            // [ceil(tokens / kPiece)][2][width]: sums of the pieces of long runs
   int64_t tokens, rows, width;
   float scale;
+  int log_lanes;            // 2^log_lanes threads per row, up to 256: a block takes 256 / that rows (or pieces) side by side
+  __host__ __device__ int lanes() const { return 1 << log_lanes; }
+  __host__ __device__ int side_by_side() const { return 256 >> log_lanes; }
+  __device__ int lane() const { return threadIdx.x & (lanes() - 1); }
+  __device__ int line() const { return threadIdx.x >> log_lanes; }
 };
 
 __device__ __forceinline__ int lower_bound(const int* keys, int count, int key) {
@@ -320,10 +325,11 @@ __device__ __forceinline__ void add_rows(float (&sum)[N], const GradientArgs& a,
   }
 }
 
-// Blocks [0, start_blocks): the rows' first tokens by search. The others: pieces (x-major) x blocks of columns. A piece
+// Blocks [0, start_blocks): the rows' first tokens by search. The others: pieces (256 / lanes each) x blocks of columns. A piece
 // holds parts of at most two long runs: the one that reaches in from before or fills it, and the one that reaches out.
 template <typename T, bool VECTOR>
 __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int start_blocks, int column_blocks) {
+  grid_dependency_wait();
   constexpr int N = VECTOR ? 8 : 1;
   const int tokens = static_cast<int>(a.tokens);
   if (static_cast<int>(blockIdx.x) < start_blocks) {
@@ -331,9 +337,10 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int
     if (row <= a.rows) a.starts[row] = lower_bound(a.keys, tokens, static_cast<int>(row));
     return;
   }
-  const int block = blockIdx.x - start_blocks, piece = block / column_blocks;
-  const int64_t column = (static_cast<int64_t>(block % column_blocks) * 256 + threadIdx.x) * N;
+  const int block = blockIdx.x - start_blocks, piece = block / column_blocks * a.side_by_side() + a.line();
+  const int64_t column = (static_cast<int64_t>(block % column_blocks) * a.lanes() + a.lane()) * N;
   const int begin = piece * kPiece, end = min(tokens, begin + kPiece);
+  if (begin >= tokens) return;
   const int head = a.keys[begin], tail = a.keys[end - 1];
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
@@ -357,24 +364,28 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int
 // (dependent) load of where their runs start is paid once: 141 us instead of 204 with a row per block, 16384 tokens on
 // 49152 x 4096.
 constexpr int kRowsPerBlock = 8;
-template <typename T, typename W, bool VECTOR>
+template <typename T, typename W, bool VECTOR, bool WIDE>
 __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a) {
+  grid_dependency_wait();
+  if constexpr (WIDE) a.log_lanes = 8;
   constexpr int N = VECTOR ? 8 : 1;
-  const int64_t column = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * N;
+  const int64_t column = (static_cast<int64_t>(blockIdx.y) * a.lanes() + a.lane()) * N;
   if (column >= a.width) return;
   W* out = static_cast<W*>(a.out) + column;
   // rows a grid's width apart: frequent tokens tend to be neighbours and should not meet in one block
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.side_by_side() + a.line();
+  const int64_t row_step = static_cast<int64_t>(gridDim.x) * a.side_by_side();
   int starts[kRowsPerBlock], ends[kRowsPerBlock];
 #pragma unroll
   for (int r = 0; r < kRowsPerBlock; ++r) {
-    const int64_t row = blockIdx.x + static_cast<int64_t>(r) * gridDim.x;
+    const int64_t row = row0 + r * row_step;
     starts[r] = row < a.rows ? a.starts[row] : 0;
     ends[r] = row < a.rows ? a.starts[row + 1] : 0;
   }
 #pragma unroll
   for (int r = 0; r < kRowsPerBlock; ++r) {
     const int first = starts[r], last = ends[r];
-    const int64_t row = blockIdx.x + static_cast<int64_t>(r) * gridDim.x;
+    const int64_t row = row0 + r * row_step;
     if (row >= a.rows) break;
     float sum[N] = {};
     if (last - first <= kPiece) {
@@ -427,7 +438,7 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
     // with the 33 KB of counters all but the smallest are above the default limit
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return fail(CT_ERR_CUDA, "embedding_sort_one_block_kernel: %s", cudaGetErrorString(err));
-    kernel<<<1, kSortThreads, smem, stream>>>(ids, static_cast<int>(tokens), rows, padding, bits, keys, positions, error_flag);
+    launch_dependent(kernel, dim3(1), dim3(kSortThreads), smem, stream, ids, static_cast<int>(tokens), rows, padding, bits, keys, positions, error_flag);
     count_launch(false);
     return check_launch("embedding_sort_one_block_kernel");
   }
@@ -441,8 +452,9 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
     const int shift = pass * kRadixBits;
     const auto count = sort_steps(tokens) == 1 ? embedding_sort_count_kernel<1> : embedding_sort_count_kernel<kManySteps>;
     const auto scatter = sort_steps(tokens) == 1 ? embedding_sort_scatter_kernel<1> : embedding_sort_scatter_kernel<kManySteps>;
-    count<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
-    scatter<<<blocks, kSortThreads, 0, stream>>>(ids, from_keys, from_positions, tokens, rows, padding, shift, histogram, to_keys, to_positions, error_flag);
+    launch_dependent(count, dim3(blocks), dim3(kSortThreads), 0, stream, ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
+    launch_dependent(scatter, dim3(blocks), dim3(kSortThreads), 0, stream, ids, from_keys, from_positions, tokens, rows, padding, shift, histogram,
+                     to_keys, to_positions, error_flag);
     for (int i = 0; i < 2; ++i) count_launch(false);
     from_keys = to_keys;
     from_positions = to_positions;
@@ -450,18 +462,22 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
   return check_launch("embedding_sort");
 }
 
-template <typename T, typename W, bool VECTOR> int gradient(const GradientArgs& a, cudaStream_t stream) {
-  const int64_t per_block = 256 * (VECTOR ? 8 : 1);
+template <typename T, typename W, bool VECTOR> int gradient(GradientArgs a, cudaStream_t stream) {
+  a.log_lanes = 0;
+  while (a.log_lanes < 8 && a.lanes() * (VECTOR ? 8 : 1) < a.width) ++a.log_lanes;
+  const int64_t per_block = a.lanes() * (VECTOR ? 8 : 1), side_by_side = a.side_by_side();
   const int64_t column_blocks = (a.width + per_block - 1) / per_block, start_blocks = (a.rows + 256) / 256;
   if (column_blocks > 65535) return fail(CT_ERR_UNSUPPORTED, "ct_embedding_gradient: width %lld", (long long)a.width);
-  const int64_t blocks = start_blocks + piece_count(a.tokens) * column_blocks;
+  const int64_t blocks = start_blocks + (piece_count(a.tokens) + side_by_side - 1) / side_by_side * column_blocks;
   if (blocks > 0x7fffffff) return fail(CT_ERR_UNSUPPORTED, "ct_embedding_gradient: %lld tokens", (long long)a.tokens);
-  embedding_runs_kernel<T, VECTOR><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a, static_cast<int>(start_blocks), static_cast<int>(column_blocks));
+  launch_dependent(embedding_runs_kernel<T, VECTOR>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, a, static_cast<int>(start_blocks),
+                   static_cast<int>(column_blocks));
   count_launch(false);
   const int rc = check_launch("embedding_runs_kernel");
   if (rc) return rc;
-  const int64_t grid = (a.rows + kRowsPerBlock - 1) / kRowsPerBlock;
-  embedding_gradient_kernel<T, W, VECTOR><<<dim3(static_cast<unsigned>(grid), static_cast<unsigned>(column_blocks)), 256, 0, stream>>>(a);
+  const int64_t grid = (a.rows + kRowsPerBlock * side_by_side - 1) / (kRowsPerBlock * side_by_side);
+  launch_dependent(a.log_lanes == 8 ? embedding_gradient_kernel<T, W, VECTOR, true> : embedding_gradient_kernel<T, W, VECTOR, false>,
+                   dim3(static_cast<unsigned>(grid), static_cast<unsigned>(column_blocks)), dim3(256), 0, stream, a);
   count_launch(false);
   return check_launch("embedding_gradient_kernel");
 }
@@ -529,7 +545,7 @@ extern "C" int ct_embedding_gradient(const void* dy, int64_t ld, const int64_t* 
   int* other_keys = reinterpret_cast<int*>(take(many ? list : 0));
   int* other_positions = reinterpret_cast<int*>(take(many ? list : 0));
   int* histogram = reinterpret_cast<int*>(take(many ? padded(sort_blocks(tokens) * kRadix * 4) : 0));
-  GradientArgs a{dy, ld, d_table, keys, positions, nullptr, nullptr, tokens, rows, width, scale};
+  GradientArgs a{dy, ld, d_table, keys, positions, nullptr, nullptr, tokens, rows, width, scale, 0};
   a.starts = reinterpret_cast<int*>(take(padded((rows + 1) * 4)));
   a.pieces = reinterpret_cast<float*>(at);
   if (tokens) {

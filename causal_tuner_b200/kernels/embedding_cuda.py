@@ -11,13 +11,16 @@ import torch
 from .. import _lib
 
 
+_INTEGERS = frozenset((torch.int64, torch.int32, torch.int16, torch.uint8))
+
+
 def _ids(ids, other):
     _lib.require_cuda(ids, other)
-    if ids.dtype not in (torch.int64, torch.int32, torch.int16, torch.uint8):
+    if ids.dtype not in _INTEGERS:
         raise TypeError(f"token ids must be integers, not {ids.dtype}")
     if ids.device != other.device:
         raise ValueError("token ids and the table must be on one device")
-    return ids.to(torch.int64).contiguous()
+    return (ids if ids.dtype == torch.int64 else ids.to(torch.int64)).contiguous()
 
 
 def embedding_lookup(ids, weight, *, scale=1.0, dtype=None):
