@@ -16,11 +16,12 @@ namespace {
 
 constexpr int kRadixBits = 8, kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-// Tokens per thread of the many-block sort: one, so that 16384 tokens are 16 blocks, four where the blocks' histograms
-// (which every block sums) would otherwise weigh more than the tokens.
-constexpr int kManySteps = 4;
-constexpr int64_t kOneStepTokens = 65536;
-constexpr int kOneBlockItems = 4 * kSortThreads;       // up to here one block sorts alone, in shared memory, in one launch
+// Up to 1024 tokens are sorted by one block in shared memory, up to 32768 by a cluster of eight blocks in one launch (which
+// counts for calls of this size: two launches per digit took the 12 thousand tokens of a small batch from 30 to 45 us),
+// more by as many blocks as it takes, two launches per digit.
+constexpr int kOneBlockItems = kSortThreads;
+constexpr int kCluster = 8, kClusterItems = 4 * kCluster * kSortThreads;
+constexpr int kManySteps = 4, kManyItems = kManySteps * kSortThreads;
 constexpr int kPiece = 32;                             // sorted tokens per piece of a long run
 constexpr int kBadToken = 9;                           // device error code
 
@@ -167,11 +168,11 @@ __device__ __forceinline__ int item_index(int k, int items_per_warp) {
   return (threadIdx.x >> 5) * items_per_warp + 32 * k + (threadIdx.x & 31);
 }
 
-template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_one_block_kernel(const int64_t* ids, int tokens, int64_t rows, int64_t padding,
                                                                                 int bits, int* keys, int* positions, int* error_flag) {
   grid_dependency_wait();
-  extern __shared__ int2 items[];                       // (key, position)
+  constexpr int STEPS = 1;
+  __shared__ int2 items[kOneBlockItems];                 // (key, position)
   __shared__ SortShared s;
   int2 mine[STEPS];
   int digit[STEPS], rank[STEPS];
@@ -235,6 +236,57 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_count_kernel(cons
   if (threadIdx.x < kRadix) histogram[static_cast<int64_t>(blockIdx.x) * kRadix + threadIdx.x] = total;
 }
 
+// The blocks' histograms -> the first place of each digit's items of this block: the items of smaller digits in all blocks,
+// and those of the digit in the blocks before. Every block sums the histograms for itself.
+__device__ __forceinline__ void place_digits(SortShared& s, const int* histogram, int blocks, int block) {
+  int total = 0, before = 0;
+  if (threadIdx.x < kRadix)
+    for (int b = 0; b < blocks; ++b) {
+      const int n = histogram[static_cast<int64_t>(b) * kRadix + threadIdx.x];
+      before += b < block ? n : 0;
+      total += n;
+    }
+  digit_sums(s, total);
+  if (threadIdx.x < kRadix) s.digit_base[threadIdx.x] += before;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The whole sort by one cluster: items and histograms go through memory, the passes are separated by cluster barriers.
+template <int STEPS>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads)
+    embedding_sort_cluster_kernel(const int64_t* ids, int64_t tokens, int64_t rows, int64_t padding, int passes, int* keys, int* positions,
+                                  int* other_keys, int* other_positions, int* histogram, int* error_flag) {
+  grid_dependency_wait();
+  __shared__ SortShared s;
+  int key[STEPS], position[STEPS], digit[STEPS], rank[STEPS];
+  load_items(key, position, ids, nullptr, nullptr, tokens, rows, padding, error_flag);
+  for (int pass = 0; pass < passes; ++pass) {
+    const bool to_first = (passes - 1 - pass) % 2 == 0;
+    int* to_keys = to_first ? keys : other_keys;
+    int* to_positions = to_first ? positions : other_positions;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> (pass * kRadixBits)) & (kRadix - 1);
+    count_digits(s, digit, rank);
+    const int total = sum_over_warps(s);
+    if (threadIdx.x < kRadix) histogram[blockIdx.x * kRadix + threadIdx.x] = total;
+    __threadfence();
+    cluster_barrier();
+    place_digits(s, histogram, kCluster, blockIdx.x);
+    hand_out(s, digit, rank, [&](int k, int at) {
+      to_keys[at] = key[k];
+      to_positions[at] = position[k];
+    });
+    __threadfence();
+    cluster_barrier();                  // also: nobody counts the next digit before all have read this one's histograms
+    if (pass + 1 < passes) load_items(key, position, ids, to_keys, to_positions, tokens, rows, padding, error_flag);
+  }
+}
+
 template <int STEPS>
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(const int64_t* ids, const int* src_keys, const int* src_positions,
                                                                               int64_t tokens, int64_t rows, int64_t padding, int shift,
@@ -247,17 +299,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_scatter_kernel(co
   for (int k = 0; k < STEPS; ++k) digit[k] = key[k] < 0 ? -1 : (key[k] >> shift) & (kRadix - 1);
   count_digits(s, digit, rank);
   sum_over_warps(s);
-  // every block sums the histogram for itself: the digit's items in all blocks, and in the blocks before this one
-  int total = 0, before = 0;
-  if (threadIdx.x < kRadix)
-    for (unsigned b = 0; b < gridDim.x; ++b) {
-      const int n = histogram[static_cast<int64_t>(b) * kRadix + threadIdx.x];
-      before += b < blockIdx.x ? n : 0;
-      total += n;
-    }
-  digit_sums(s, total);
-  if (threadIdx.x < kRadix) s.digit_base[threadIdx.x] += before;
-  __syncthreads();
+  place_digits(s, histogram, gridDim.x, blockIdx.x);
   hand_out(s, digit, rank, [&](int k, int at) {
     keys[at] = key[k];
     positions[at] = position[k];
@@ -410,8 +452,7 @@ __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a)
 bool known(int dtype) { return dtype == CT_F32 || dtype == CT_BF16 || dtype == CT_F16; }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-int sort_steps(int64_t tokens) { return tokens <= kOneStepTokens ? 1 : kManySteps; }
-int64_t sort_blocks(int64_t tokens) { return (tokens + sort_steps(tokens) * kSortThreads - 1) / (sort_steps(tokens) * kSortThreads); }
+int64_t sort_blocks(int64_t tokens) { return tokens <= kClusterItems ? kCluster : (tokens + kManyItems - 1) / kManyItems; }
 int64_t piece_count(int64_t tokens) { return (tokens + kPiece - 1) / kPiece; }
 
 template <typename F> int by_type(int dtype, F f) {
@@ -431,16 +472,19 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
                 int* other_positions, int* histogram, int* error_flag, cudaStream_t stream) {
   const int bits = bits_of(rows), passes = (bits + kRadixBits - 1) / kRadixBits;
   if (tokens <= kOneBlockItems) {
-    // 1 or 4 tokens a thread (with 16, one block takes 51 us for 16384 tokens, many blocks half of that)
-    const int steps = tokens <= kSortThreads ? 1 : 4;
-    const auto kernel = steps == 1 ? embedding_sort_one_block_kernel<1> : embedding_sort_one_block_kernel<4>;
-    const int smem = steps * kSortThreads * static_cast<int>(sizeof(int2));
-    // with the 33 KB of counters all but the smallest are above the default limit
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (err != cudaSuccess) return fail(CT_ERR_CUDA, "embedding_sort_one_block_kernel: %s", cudaGetErrorString(err));
-    launch_dependent(kernel, dim3(1), dim3(kSortThreads), smem, stream, ids, static_cast<int>(tokens), rows, padding, bits, keys, positions, error_flag);
+    launch_dependent(embedding_sort_one_block_kernel, dim3(1), dim3(kSortThreads), 0, stream, ids, static_cast<int>(tokens), rows, padding, bits,
+                     keys, positions, error_flag);
     count_launch(false);
     return check_launch("embedding_sort_one_block_kernel");
+  }
+  if (tokens <= kClusterItems) {
+    const auto kernel = tokens <= kClusterItems / 4   ? embedding_sort_cluster_kernel<1>
+                        : tokens <= kClusterItems / 2 ? embedding_sort_cluster_kernel<2>
+                                                      : embedding_sort_cluster_kernel<4>;
+    launch_dependent(kernel, dim3(kCluster), dim3(kSortThreads), 0, stream, ids, tokens, rows, padding, passes, keys, positions, other_keys,
+                     other_positions, histogram, error_flag);
+    count_launch(false);
+    return check_launch("embedding_sort_cluster_kernel");
   }
   const unsigned blocks = static_cast<unsigned>(sort_blocks(tokens));
   const int* from_keys = nullptr;
@@ -450,8 +494,8 @@ int sort_tokens(const int64_t* ids, int64_t tokens, int64_t rows, int64_t paddin
     int* to_keys = last_is_first ? keys : other_keys;
     int* to_positions = last_is_first ? positions : other_positions;
     const int shift = pass * kRadixBits;
-    const auto count = sort_steps(tokens) == 1 ? embedding_sort_count_kernel<1> : embedding_sort_count_kernel<kManySteps>;
-    const auto scatter = sort_steps(tokens) == 1 ? embedding_sort_scatter_kernel<1> : embedding_sort_scatter_kernel<kManySteps>;
+    const auto count = embedding_sort_count_kernel<kManySteps>;
+    const auto scatter = embedding_sort_scatter_kernel<kManySteps>;
     launch_dependent(count, dim3(blocks), dim3(kSortThreads), 0, stream, ids, from_keys, tokens, rows, padding, shift, histogram, error_flag);
     launch_dependent(scatter, dim3(blocks), dim3(kSortThreads), 0, stream, ids, from_keys, from_positions, tokens, rows, padding, shift, histogram,
                      to_keys, to_positions, error_flag);

@@ -59,7 +59,8 @@ def check_gradient(ids, dy, rows, scale=1.0, padding_idx=None, dtype=torch.float
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("kind", ["uniform", "skewed", "same", "two", "sorted", "reverse"])
 @pytest.mark.parametrize("tokens, rows, width", [(1, 1, 1), (7, 97, 33), (128, 5, 32), (129, 300, 40), (1000, 1000, 256),
-                                                 (4097, 70000, 24), (16384, 3, 16), (16385, 300, 24), (40000, 1 << 17, 8)])
+                                                 (1024, 5000, 8), (1025, 5000, 8), (4097, 70000, 24), (8193, 1 << 17, 8),
+                                                 (16384, 3, 16), (16385, 300, 24), (32768, 70000, 8), (32769, 70000, 8), (40000, 1 << 17, 8)])
 def test_gradient(dtype, kind, tokens, rows, width):
     check_gradient(make_ids(tokens, rows, kind), make_dy(tokens, width, dtype), rows)
 

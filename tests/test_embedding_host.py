@@ -25,8 +25,8 @@ def test_workspace():
     size = _lib.load().ct_embedding_gradient_workspace
     # two lists of 1000 tokens, 11 run starts, 32 pieces x 2 rows of 16 floats
     assert size(1000, 10, 16) == 2 * 4096 + 256 + 4096
-    # above 4096 tokens four lists and the blocks' histograms
-    assert size(20000, 10, 16) == 4 * 80128 + 20 * 256 * 4 + 256 + 625 * 2 * 64 + 128
+    # above 1024 tokens four lists and the blocks' histograms
+    assert size(20000, 10, 16) == 4 * 80128 + 8 * 256 * 4 + 256 + 625 * 2 * 64 + 128
 
 
 def test_no_cpu_path():
