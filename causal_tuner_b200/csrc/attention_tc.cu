@@ -442,18 +442,18 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
         for (int j = 0; j < w.n && alive; ++j) {
           const int t = t0 + j, r = t % RING, next = (t + 1) % RING;
           const uint32_t next_parity = ((t + 1) / RING) & 1;
-          if (!wait.warp(v_full(r), (t / RING) & 1, 7)) { alive = false; break; }
+          // a wait costs this warp 150 cycles even where nothing is to wait for: those for the copies go with others
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const int count = w.count(s);
             if (j < count) {
-              if (!wait.warp(p_full(s, 0), tiles[s] & 1, 7)) { alive = false; break; }
+              if (!(s == 0 || j >= w.n0 ? wait.both(v_full(r), (t / RING) & 1, p_full(s, 0), tiles[s] & 1, 7) : wait.warp(p_full(s, 0), tiles[s] & 1, 7))) { alive = false; break; }
               tcgen05_fence_after();
               product_tn<T, HD, 8, 64, 0, 4>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, j > 0);
               commit(half_done(s));
               ++tiles[s];
               if (w.both_halves(s, j)) {
-                if (!wait.warp(p_full(s, 1), halves[s] & 1, 7)) { alive = false; break; }
+                if (!(s == 0 && j + 1 < w.n ? wait.both(k_full(next), next_parity, p_full(s, 1), halves[s] & 1, 7) : wait.warp(p_full(s, 1), halves[s] & 1, 7))) { alive = false; break; }
                 ++halves[s];
                 tcgen05_fence_after();
                 product_tn<T, HD, 8, 64, 4, 8>(tmem + kOutColumn + s * 128, tmem + s * 128, v_ring + r * TILE, true);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
             }
             if (s == 1) commit(v_empty(r));
             if (j + 1 < w.n) {
-              if (s == 0 && !wait.warp(k_full(next), next_parity, 7)) { alive = false; break; }
+              if (s == 0 && !(j < count && w.both_halves(s, j)) && !wait.warp(k_full(next), next_parity, 7)) { alive = false; break; }
               if (j + 1 < count) scores(w, s, j + 1, t + 1);
               if (s == 1) commit(k_empty(next));
             } else if (following.valid()) {                        // the next unit's first scores
