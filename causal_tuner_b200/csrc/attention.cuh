@@ -39,7 +39,7 @@ struct HeadsView {          // [tokens, heads, head_dim], innermost stride 1
 struct AttentionArgs {
   HeadsView q, k, v;
   void* out;                // [tokens, heads, head_dim] contiguous
-  float* lse;               // [tokens, heads]: log2 of the sum of exp over the row's scaled scores, times 1 (base 2)
+  float* lse;               // [tokens, heads]: log2 of the sum over the row's keys of exp(scaled score)
   const void* dy;           // backward: [tokens, heads, head_dim] contiguous
   float* delta;             // backward: [tokens, heads] workspace, sum over the channels of dy * out
   void* dq;                 // contiguous, as out

@@ -3,6 +3,8 @@
 //   forward   x[t] = round(scale * table[id[t]])
 //   gradient  d_table[i] = scale * sum over the tokens t with id[t] = i, in order of t, of dy[t]; zero rows elsewhere
 //
+// The lookup is bound by memory: 69 us for 16384 tokens out of a 49152 x 4096 fp32 table to bf16 (5.2 TB/s of the 363 MB
+// that have to move, 0.80 of a plain copy).
 // The gradient is bound by its dense result: every row is written once, 805 MB for 49152 x 4096 in fp32, of which 16384
 // tokens touch a quarter. So nothing is cleared beforehand and nothing is accumulated in memory: the tokens are sorted by id
 // (stable radix sort, a few us), every row knows its run of tokens and one kernel writes zeros, single rows and sums.
@@ -16,9 +18,9 @@ namespace {
 
 constexpr int kRadixBits = 8, kRadix = 1 << kRadixBits;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-// Up to 1024 tokens are sorted by one block in shared memory, up to 32768 by a cluster of eight blocks in one launch (which
-// counts for calls of this size: two launches per digit took the 12 thousand tokens of a small batch from 30 to 45 us),
-// more by as many blocks as it takes, two launches per digit.
+// Up to 1024 tokens are sorted by one block in shared memory, up to 32768 by a cluster of eight blocks in one launch (for
+// calls of this size launches count: 12 thousand tokens on a narrow table take 32 us, 45 with two launches per digit), more
+// by as many blocks as it takes, two launches per digit.
 constexpr int kOneBlockItems = kSortThreads;
 constexpr int kCluster = 8, kClusterItems = 4 * kCluster * kSortThreads;
 constexpr int kManySteps = 4, kManyItems = kManySteps * kSortThreads;
@@ -403,8 +405,8 @@ __global__ void __launch_bounds__(256) embedding_runs_kernel(GradientArgs a, int
 }
 
 // Every row of the table, every column: zeros, or the sum of the row's run. A block takes kRowsPerBlock rows so that the
-// (dependent) load of where their runs start is paid once: 141 us instead of 204 with a row per block, 16384 tokens on
-// 49152 x 4096.
+// (dependent) load of where their runs start is paid once: 158 us instead of 204 with a row per block, 16384 tokens on
+// 49152 x 4096 (940 MB: 143 us at the rate of a plain copy); the whole gradient takes 178 us, sort and runs included.
 constexpr int kRowsPerBlock = 8;
 template <typename T, typename W, bool VECTOR, bool WIDE>
 __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a) {

@@ -509,7 +509,7 @@ CT_API int ct_attention_backward(const void* q, int64_t q_token, int64_t q_head,
                                  float scale, int dtype, int path, void* workspace, void* stream);
 
 /* ---- token embedding ----------------------------------------------------------------
- * Stand in for nn.Embedding and its cast in the decoder (modeling/model.py:160-165,229 of the reference), and for its
+ * Stand in for nn.Embedding and its cast in the decoder (modeling/model.py:227 of the reference), and for its
  * backward pass when the embedding trains (modeling/model.py:185-193).
  * ct_embedding_forward: out[t, :] = round(scale * table[ids[t], :]) in `out_dtype`; table [rows, width] contiguous.
  * ct_embedding_gradient: d_table[i, :] = scale * sum of dy[t, :] over the tokens with ids[t] == i, in fp32 in the order of
