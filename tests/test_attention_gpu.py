@@ -268,6 +268,46 @@ def test_on_another_stream_and_in_a_graph(dtype):
             assert all(torch.equal(a, b) for a, b in zip(outputs, results.values()))
 
 
+@pytest.mark.parametrize("heads, kv_heads", [(128, 1), (128, 128)])
+def test_offsets_above_32_bits(heads, kv_heads):
+    """More than 2^31 elements of q: the last documents come out as they do alone."""
+    rows, width, dim = 137, 1024, 128
+    assert rows * width * heads * dim > 2 ** 31
+    generator = torch.Generator(device="cuda").manual_seed(3)
+    make = lambda h: torch.randn(rows, width, h, dim, generator=generator, device="cuda", dtype=torch.bfloat16)
+    q, k, v, dy = make(heads), make(kv_heads), make(kv_heads), make(heads)
+    spans = tuple((row, start, start + 64) for row in range(rows) for start in range(0, width, 64))
+    actual = run(q, k, v, dy, spans)
+    for row in (0, rows - 1):
+        alone = run(*(t[row:row + 1].clone() for t in (q, k, v, dy)), tuple((0, start, start + 64) for start in range(0, width, 64)))
+        for name in ("y", "dq"):
+            assert torch.equal(actual[name][row], alone[name][0]), name
+        for name in ("dk", "dv"):             # pieces depend on the whole batch, so the order of sums does
+            a, b = actual[name][row].double(), alone[name][0].double()
+            assert float((a - b).norm()) <= 2.0 ** -8 * float(b.norm()), name
+
+
+def test_two_host_threads_at_once():
+    inputs = [tensors(2, 500, 8, 1, 64, "bf16", seed=i) for i in range(2)]
+    spans = [documents(2, 500, i, 300, gap=3) for i in range(2)]
+    expected = [run(*inputs[i], spans[i]) for i in range(2)]
+    torch.cuda.synchronize()
+    results = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                results[i] = run(*inputs[i], spans[i])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    for i in range(2):
+        assert all(torch.equal(results[i][name], expected[i][name]) for name in expected[i])
+
+
 def test_a_plan_may_be_dropped_once_the_calls_are_issued():
     spans = documents(2, 700, 4, 300, gap=3)
     q, k, v, dy = tensors(2, 700, 8, 1, 64, "bf16")

@@ -177,6 +177,20 @@ def test_on_another_stream_and_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(results, expected))
 
 
+def test_offsets_above_32_bits():
+    rows, width = (1 << 20) + 5, 2056
+    assert rows * width > 2 ** 31
+    weight = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    ids = torch.tensor([rows - 1, 3, rows - 1, rows - 2, 0], device="cuda")
+    weight[ids] = torch.arange(5 * width, device="cuda").view(5, width).remainder(200).to(torch.bfloat16)
+    assert torch.equal(embedding_lookup(ids, weight), weight[ids])
+    dy = make_dy(5, width, "bf16")
+    grad = embedding_gradient(dy, ids, rows, dtype=torch.bfloat16)
+    assert torch.equal(grad[rows - 1], (dy[0].float() + dy[2].float()).to(torch.bfloat16))
+    assert torch.equal(grad[rows - 2], dy[3]) and torch.equal(grad[3], dy[1]) and torch.equal(grad[0], dy[4])
+    assert int((grad != 0).any(1).sum()) == 4
+
+
 def test_refusals():
     weight, ids, dy = make_dy(10, 16, "fp32"), make_ids(4, 10, "uniform"), make_dy(4, 16, "fp32")
     with pytest.raises(TypeError, match="integers"):
