@@ -527,6 +527,7 @@ extern "C" int ct_attention_forward(const void* q, int64_t q_token, int64_t q_he
   a.out = out;
   a.lse = lse;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (path == CT_PATH_AUTO) path = attention_tc_supported(a) ? CT_PATH_TCGEN05 : CT_PATH_SIMT;
   rc = check_path(a, "ct_attention_forward", path);
   if (rc) return rc;
   const int64_t row = static_cast<int64_t>(heads) * head_dim * dtype_size(dtype);

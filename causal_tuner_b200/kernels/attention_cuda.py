@@ -184,10 +184,9 @@ def attention_forward(q, k, v, plan, *, scale=None, keep_lse=True):
     library, code = _lib.load(), _lib.code_of(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q):
-        path = _path(library, operands, heads, plan.kv_heads, dim, scale, code)
         _lib.check(library.ct_attention_forward(
             *operands, out.data_ptr(), _lib.pointer(lse), plan.table.data_ptr(), plan.host_sections, tokens, heads, plan.kv_heads,
-            dim, scale, code, path, _stream(plan, q)))
+            dim, scale, code, _lib.PATH_SIMT if _lib.gemm_path == _lib.PATH_SIMT else _lib.PATH_AUTO, _stream(plan, q)))
     return out, lse
 
 

@@ -55,7 +55,7 @@ enum { CT_PATH_AUTO = 0, CT_PATH_SIMT = 1, CT_PATH_TCGEN05 = 2 };
 CT_API int ct_abi_version(void);
 /* Kernels launched by this library in this process so far (all devices). */
 CT_API int64_t ct_launch_count(void);
-/* Kernels among those that were the tcgen05 GEMM. */
+/* Kernels among those that run on tcgen05: the GEMM family and the document attention. */
 CT_API int64_t ct_tcgen05_launch_count(void);
 /* Synchronises `stream`, then returns CT_OK, or CT_ERR_DEVICE when a kernel on
  * the current device gave up on a bounded wait since the last call (the flag is
@@ -489,8 +489,9 @@ CT_API int ct_adamw_update(int count, void* const* grads, void* const* params, v
  *   5 runs of tokens of no document: (first token, count, 0, 0)
  * with tile_tokens = ct_attention_tile_tokens(heads, kv_heads). Every record must lie inside the batch: the table is
  * trusted (causal_tuner_b200.kernels.attention_cuda.prepare_documents builds it).
- * `path` is CT_PATH_TCGEN05 or CT_PATH_SIMT, as ct_attention_path answers for the operands; out, dy and the gradients
- * are 16-byte aligned for the former. Sums have a fixed order on both: repeated calls are bit-identical.
+ * `path` is CT_PATH_TCGEN05 or CT_PATH_SIMT, as ct_attention_path answers for the operands (the workspace of the
+ * backward pass depends on it; the forward pass also takes CT_PATH_AUTO); out, dy and the gradients are 16-byte aligned
+ * for the former. Sums have a fixed order on both: repeated calls are bit-identical.
  * `key_slots` = the number of slots that section 2 names. */
 CT_API int ct_attention_tile_tokens(int heads, int kv_heads);
 CT_API int ct_attention_path(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
