@@ -65,6 +65,7 @@ SIGNATURES = {
     "ct_grad_norm_workspace": (_L, [_I]),
     "ct_grad_norm": (_I, [_I, _P, _P, _P, _F, _P, _P, _P]),
     "ct_attention_tile_tokens": (_I, [_I, _I]),
+    "ct_attention_plan": (_L, [_P, _P, _L, _L, _I, _I, _P, _L, _P, _P]),
     "ct_attention_path": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _F, _I]),
     "ct_attention_forward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _L, _I, _I, _I, _F, _I, _I, _P]),
     "ct_attention_backward_workspace": (_L, [_L, _I, _I, _I, _L, _I]),

@@ -16,13 +16,11 @@ A NaN or infinity outside the documents reaches nothing; one inside a document r
 import ctypes
 from dataclasses import dataclass, field
 
-import numpy
 import torch
 
 from .. import _lib
 
 KEY_TILE = 128              # keys of one piece of the key-gradient pass (include/ct_b200.h)
-_PIECES_PER_SM, _SMS, _SMALLEST_PIECE = 4, 148, 16
 
 
 @dataclass(frozen=True)
@@ -39,45 +37,6 @@ class DocumentPlan:
     stream: int = 0                 # raw handle of the stream on which the table was made
 
 
-def _tiles(starts, lengths, step):
-    """(document, first token) of every tile of `step` tokens."""
-    counts = -(-lengths // step)
-    document = numpy.repeat(numpy.arange(len(lengths)), counts)
-    first = numpy.arange(len(document)) - numpy.repeat(numpy.cumsum(counts) - counts, counts)
-    return document, first * step
-
-
-def _query_section(starts, lengths, step):
-    document, first = _tiles(starts, lengths, step)
-    keys = numpy.minimum(first + step, lengths[document])       # a query tile's work: the keys it sees
-    order = numpy.argsort(-keys, kind="stable")
-    document, first = document[order], first[order]
-    return numpy.stack((starts[document], lengths[document], first, numpy.zeros_like(first)), 1)
-
-
-def _key_sections(starts, lengths, tile_tokens, head_blocks, kv_heads):
-    """Pieces of the key tiles and the sums over them. A key tile's queries are all later tokens of the document, so the
-    work of the tiles differs by the document's length: tiles are cut into pieces of at most a fraction of an SM's share
-    (but no smaller than _SMALLEST_PIECE query tiles, whose cost covers that of writing and adding a share)."""
-    document, first_key = _tiles(starts, lengths, KEY_TILE)
-    work = -(-(lengths[document] - first_key) // tile_tokens) * head_blocks
-    largest = max(_SMALLEST_PIECE, -(-int(work.sum()) * kv_heads // (_SMS * _PIECES_PER_SM)))
-    pieces = -(-work // largest)
-    tile = numpy.repeat(numpy.arange(len(work)), pieces)
-    index = numpy.arange(len(tile)) - numpy.repeat(numpy.cumsum(pieces) - pieces, pieces)
-    first, last = work[tile] * index // pieces[tile], work[tile] * (index + 1) // pieces[tile]
-    split = pieces > 1
-    slots = numpy.where(split, pieces, 0)
-    first_slot = numpy.cumsum(slots) - slots
-    slot = numpy.where(split[tile], first_slot[tile] + index, -1)
-    order = numpy.argsort(-(last - first), kind="stable")
-    zero = numpy.zeros_like(tile)
-    records = numpy.stack((starts[document][tile], lengths[document][tile], first_key[tile], slot, first, last, zero, zero), 1)
-    rows = numpy.minimum(KEY_TILE, lengths[document] - first_key)
-    sums = numpy.stack((starts[document] + first_key, rows, first_slot, slots), 1)[split]
-    return records[order].reshape(-1, 4), sums, int(slots.sum())
-
-
 def prepare_documents(shape, spans, device, heads, kv_heads=1):
     """The plan of a [rows, width] batch whose documents are `spans`, ((row, start, end), ...) as `segments.runs` gives
     them: any order, gaps allowed, no token in two documents. A captured graph reads the plan's table when it is replayed:
@@ -85,37 +44,31 @@ def prepare_documents(shape, spans, device, heads, kv_heads=1):
     rows, width = (int(n) for n in shape)
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads cannot share {kv_heads} key heads")
+    tokens = rows * width
+    if tokens >= 2 ** 31 - 256:
+        raise NotImplementedError(f"{tokens} tokens in one batch")
     spans = tuple(spans)
-    table = numpy.array(spans, dtype=numpy.int64).reshape(len(spans), 3)
-    row, start, end = table[:, 0], table[:, 1], table[:, 2]
-    if ((row < 0) | (row >= rows) | (start < 0) | (end < start) | (end > width)).any():
-        raise ValueError("a document span lies outside the batch")
-    if rows * width >= 2 ** 31 - 256:
-        raise NotImplementedError(f"{rows * width} tokens in one batch")
-    starts, lengths = row * width + start, end - start
-    starts, lengths = starts[lengths > 0], lengths[lengths > 0]
-    order = numpy.argsort(starts, kind="stable")
-    starts, lengths = starts[order], lengths[order]
-    ends = starts + lengths
-    if (starts[1:] < ends[:-1]).any():
-        raise ValueError("document spans overlap")
-    tile_tokens = _lib.load().ct_attention_tile_tokens(heads, kv_heads)
-    head_blocks = heads // kv_heads * tile_tokens // 128
-    keys, sums, slots = _key_sections(starts, lengths, tile_tokens, head_blocks, kv_heads)
-    gap_start = numpy.concatenate(([0], ends))
-    gap_length = numpy.concatenate((starts, [rows * width])) - gap_start
-    gap_start, gap_length = gap_start[gap_length > 0], gap_length[gap_length > 0]
-    run, offset = _tiles(gap_start, gap_length, 64)
-    zero = numpy.zeros_like(offset)
-    gaps = numpy.stack((gap_start[run] + offset, numpy.minimum(64, gap_length[run] - offset), zero, zero), 1)
-    parts = (_query_section(starts, lengths, 2 * tile_tokens), _query_section(starts, lengths, tile_tokens), keys, sums,
-             _query_section(starts, lengths, KEY_TILE), gaps)
-    first = numpy.cumsum([0] + [len(part) for part in parts])
-    sections = tuple((int(first[i]), len(part) // 2 if i == 2 else len(part)) for i, part in enumerate(parts))
-    records = numpy.ascontiguousarray(numpy.concatenate(parts), dtype=numpy.int32)
-    host = (ctypes.c_int64 * 12)(*(n for pair in sections for n in pair))
-    table = torch.from_numpy(records).to(device)
-    return DocumentPlan((rows, width), heads, kv_heads, spans, table, sections, slots, host,
+    for row, start, end in spans:
+        if not (0 <= row < rows and 0 <= start <= end <= width):
+            raise ValueError(f"the document span {(row, start, end)} lies outside the batch")
+    count = len(spans)
+    starts = (ctypes.c_int64 * count)(*[row * width + start for row, start, _ in spans])
+    lengths = (ctypes.c_int64 * count)(*[end - start for _, start, end in spans])
+    library = _lib.load()
+    tile_tokens = library.ct_attention_tile_tokens(heads, kv_heads)
+    # at least the records there can be: query tiles of three sizes, key pieces (two records each), sums, gaps
+    capacity = 2 * tokens // tile_tokens + tokens // 16 + 10 * count + 2048
+    records = torch.empty((capacity, 4), dtype=torch.int32)
+    host, slots = (ctypes.c_int64 * 12)(), ctypes.c_int64()
+    used = library.ct_attention_plan(starts, lengths, count, tokens, heads, kv_heads, records.data_ptr(), capacity, host,
+                                     ctypes.byref(slots))
+    if used < 0:
+        _lib.check(used)
+    if used > capacity:
+        raise RuntimeError(f"the plan has {used} records, room was made for {capacity}")
+    table = records[:used].to(device, copy=True)
+    sections = tuple((host[2 * i], host[2 * i + 1]) for i in range(6))
+    return DocumentPlan((rows, width), heads, kv_heads, spans, table, sections, slots.value, host,
                         _lib.stream_of(table) if table.is_cuda else 0)
 
 

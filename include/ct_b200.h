@@ -488,12 +488,18 @@ CT_API int ct_adamw_update(int count, void* const* grads, void* const* params, v
  *   4 tiles of 128 tokens for the shape-generic kernels, a = first token
  *   5 runs of tokens of no document: (first token, count, 0, 0)
  * with tile_tokens = ct_attention_tile_tokens(heads, kv_heads). Every record must lie inside the batch: the table is
- * trusted (causal_tuner_b200.kernels.attention_cuda.prepare_documents builds it).
+ * trusted (ct_attention_plan builds it).
  * `path` is CT_PATH_TCGEN05 or CT_PATH_SIMT, as ct_attention_path answers for the operands (the workspace of the
  * backward pass depends on it; the forward pass also takes CT_PATH_AUTO); out, dy and the gradients are 16-byte aligned
  * for the former. Sums have a fixed order on both: repeated calls are bit-identical.
  * `key_slots` = the number of slots that section 2 names. */
 CT_API int ct_attention_tile_tokens(int heads, int kv_heads);
+/* Builds that table on the host: `starts` / `lengths` (HOST) are the documents in the flattened batch, in any order, without
+ * overlap. Returns the number of records (or a negative CT_ERR_*) and fills the twelve `sections` and `key_slots`;
+ * `table` (HOST, room for `capacity` records) is filled as far as whole sections fit. */
+CT_API int64_t ct_attention_plan(const int64_t* starts, const int64_t* lengths, int64_t documents, int64_t tokens,
+                                 int heads, int kv_heads, int32_t* table, int64_t capacity, int64_t* sections,
+                                 int64_t* key_slots);
 CT_API int ct_attention_path(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                              int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int heads, int kv_heads,
                              int head_dim, float scale, int dtype);

@@ -86,6 +86,32 @@ def test_refused_spans_and_heads():
         prepare_documents((2 ** 16, 2 ** 15), (), "cpu", 4)
 
 
+def test_plan_entry_point():
+    library = _lib.load()
+    pair = lambda *values: (ctypes.c_int64 * len(values))(*values)
+    sections, slots = (ctypes.c_int64 * 12)(), ctypes.c_int64(-1)
+
+    def plan(starts, lengths, tokens=100, heads=4, kv_heads=1, table=None, capacity=0, sections=sections):
+        return library.ct_attention_plan(pair(*starts), pair(*lengths), len(starts), tokens, heads, kv_heads, table, capacity,
+                                         sections, ctypes.byref(slots))
+    need = plan((50, 0), (50, 40))
+    # forward tiles of 64 tokens, query tiles of 32, key pieces (two records), no sums, 128-token tiles, one gap
+    assert [sections[i] for i in range(12)] == [0, 2, 2, 4, 6, 2, 10, 0, 10, 2, 12, 1] and need == 13 and slots.value == 0
+    table = (ctypes.c_int32 * (4 * need + 4))(*[-7] * (4 * need + 4))
+    assert plan((50, 0), (50, 40), table=table, capacity=need) == need
+    assert list(table[:8]) == [50, 50, 0, 0, 0, 40, 0, 0] and list(table[48:56]) == [40, 10, 0, 0, -7, -7, -7, -7]
+    table = (ctypes.c_int32 * 16)(*[-7] * 16)
+    assert plan((50, 0), (50, 40), table=table, capacity=3) == need          # only what fits is written
+    assert table[12] == -7
+    assert plan((0, 10), (11, 5)) == _lib.ERR_ARG and b"overlap" in library.ct_last_error()
+    assert plan((90,), (11,)) == _lib.ERR_ARG and b"outside" in library.ct_last_error()
+    assert plan((0,), (-1,)) == _lib.ERR_ARG
+    assert plan((0,), (5,), heads=4, kv_heads=3) == _lib.ERR_ARG
+    assert plan((0,), (5,), tokens=2 ** 31) == _lib.ERR_UNSUPPORTED
+    assert plan((0,), (5,), sections=None) == _lib.ERR_ARG
+    assert plan((), (), tokens=0) == 0
+
+
 def test_no_cpu_path():
     plan = prepare_documents((1, 4), ((0, 0, 4),), "cpu", 2)
     x = torch.zeros(1, 4, 2, 8, dtype=torch.bfloat16)
