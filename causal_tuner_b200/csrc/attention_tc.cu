@@ -131,6 +131,8 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ PlanRecord uniform(PlanRecord r) { return {uniform(r.start), uniform(r.length), uniform(r.a), uniform(r.b)}; }
 
+// MMAs of one thread execute in the order of issue; where an accumulator takes the place of an operand in TMEM (S over P,
+// S over dS), nothing else orders the two.
 // The MMA warp walks its loops as a whole - with uniform control flow descriptors stay in uniform registers, and a chain
 // of MMAs costs few instructions each - and one elected lane issues. (With one lane in the loop an MMA took 110 cycles to issue.)
 // scores: D[128, 128] = A[128, HD] . B[128, HD]^T, both tiles as 128-row boxes of 64 channels. Always all 128 columns: with
@@ -255,7 +257,7 @@ __device__ __forceinline__ void settle(const volatile int* abort_flag) {
   while (global_timer_ns() - start < 1000000ull) __nanosleep(1000);
 }
 
-// The kernels are persistent, one CTA per SM: copies and first products of a CTA's next tile of queries (or keys) run
+// The forward and the query-gradient kernel are persistent, one CTA per SM: copies and first products of a CTA's next unit run
 // under the tail of the last one, which pays where documents are short (a CTA per tile spent 4 to 6 us on starting, the
 // first copies and the end, as much as 500 keys of work). Units are sorted by falling work and dealt back and forth, so
 // that the CTAs' sums come out even.
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
     const float2 c2 = make_float2(c, c);
     // A unit's output is stored behind the next unit's first exponentials: the last P V is complete by then.
     bool pending = false;
-    int finished = 0, release_v = -1;
+    int finished = 0;
     int64_t out_row = -1;
     float out_top = 0.0f, out_sum = 0.0f;
     auto store = [&]() {
@@ -539,95 +541,93 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
       const int end = first < here.length ? min(here.length, first + p.tile_tokens) : 0, count = (end + KEYS - 1) / KEYS;
       const int token = first + thread / p.packed;
       const int last_key = min(token, here.length - 1);
-      const bool last_stage = s == (here.a + p.tile_tokens < here.length ? 1 : 0);
-      // idle in this unit: what the unit's other stage waits for must not wait for the next one
-      if (!count && pending && !store()) { alive = false; break; }
-    for (int j = 0; j < count && alive; ++j, ++tiles) {
-      const int cols = end > j * KEYS + 64 ? KEYS : 64, t = t0 + j;      // the halves this tile needs
-      const bool partial = j * KEYS + cols - 1 > first;
-      const int limit = last_key - j * KEYS;                   // columns above it are not this row's
-      if (!wait.warp(s_full(s), tiles & 1, 8)) { alive = false; break; }
-      tcgen05_fence_after();
-      if (j * KEYS + cols > here.length) {
-        // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
-        if (!wait.warp(v_full(t % RING), (t / RING) & 1, 8)) { alive = false; break; }
-        clear_rows<BOXES>(v_ring + (t % RING) * TILE, here.length - j * KEYS, cols, thread, 128);
-      }
-      // Halves of 64 keys: the first half of P V runs under the exponentials of the second. The exponentials do not wait
-      // for the half's maximum: they use the maximum so far, and the half is done again with the new one in the rare
-      // case that a score is more than 2^8 above it.
+      if (!count && pending && !store()) { alive = false; break; }       // idle in this unit: nothing to store behind
+      for (int j = 0; j < count && alive; ++j, ++tiles) {
+        const int cols = end > j * KEYS + 64 ? KEYS : 64, t = t0 + j;      // the halves this tile needs
+        const bool partial = j * KEYS + cols - 1 > first;
+        const int limit = last_key - j * KEYS;                   // columns above it are not this row's
+        if (!wait.warp(s_full(s), tiles & 1, 8)) { alive = false; break; }
+        tcgen05_fence_after();
+        if (j * KEYS + cols > here.length) {
+          // the tile runs past the document: rows of V behind its end must not meet the zero probabilities
+          if (!wait.warp(v_full(t % RING), (t / RING) & 1, 8)) { alive = false; break; }
+          clear_rows<BOXES>(v_ring + (t % RING) * TILE, here.length - j * KEYS, cols, thread, 128);
+        }
+        // Halves of 64 keys: the first half of P V runs under the exponentials of the second. The exponentials do not wait
+        // for the half's maximum: they use the maximum so far, and the half is done again with the new one in the rare
+        // case that a score is more than 2^8 above it.
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {                            // (rolled: the MMA warp shares the instruction cache)
-        if (64 * h >= cols) break;
-        uint32_t x[2][32];
+        for (int h = 0; h < 2; ++h) {                            // (rolled: the MMA warp shares the instruction cache)
+          if (64 * h >= cols) break;
+          uint32_t x[2][32];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 64 * h + 32 * g, x[g]);
+          for (int g = 0; g < 2; ++g) tmem_load_32_issue(s_addr + 64 * h + 32 * g, x[g]);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) tmem_load_wait(x[g]);
-        if (partial) {
-          rare();
+          for (int g = 0; g < 2; ++g) tmem_load_wait(x[g]);
+          if (partial) {
+            rare();
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (64 * h + 32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
-        }
-        if (j == 0 && h == 0) {                                // key 0 is every row's: a score, not -infinity
-          rare();
-          top = -INFINITY;
-          sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top = max3(top, __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
-        }
-        uint32_t packed[32];
-        float2 part[2];
-        while (true) {
-          const float shift = kLift - top * c;
-          const float2 shift2 = make_float2(shift, shift);
-          float peak[4] = {top, top, top, top};
-          part[0] = part[1] = make_float2(0.0f, 0.0f);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 raw = make_float2(__uint_as_float(x[i / 16][2 * (i % 16)]), __uint_as_float(x[i / 16][2 * (i % 16) + 1]));
-            peak[i & 3] = max3(peak[i & 3], raw.x, raw.y);
-            float2 e = fma2(raw, c2, shift2);
-            e.x = exp2_approx(e.x);
-            e.y = exp2_approx(e.y);
-            part[i & 1] = add2(part[i & 1], e);
-            packed[i] = pack2<T>(e.x, e.y);
+              for (int i = 0; i < 32; ++i)
+                if (64 * h + 32 * g + i > limit) x[g][i] = 0xff800000u;     // -infinity
           }
-          const float best = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
-          if (!__any_sync(0xffffffffu, (best - top) * c > 8.0f)) break;
-          rare();
-          // O holds the products of all halves so far; the last one issued has to be complete
-          const bool issued = h == 1 || j > 0;
-          if (h == 1 && !wait.warp(half_done(s), tiles & 1, 8)) { alive = false; break; }
-          tcgen05_fence_after();
-          const float factor = exp2_approx((top - best) * c);
-          top = best;
-          sum *= factor;
-          if (issued) {
-#pragma unroll 1
-            for (int g = 0; g < HD / 32; ++g) {
-              uint32_t o[32];
-              tmem_load_32(o_addr + 32 * g, o);
+          if (j == 0 && h == 0) {                                // key 0 is every row's: a score, not -infinity
+            rare();
+            top = -INFINITY;
+            sum = 0.0f;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-              tmem_store_32(o_addr + 32 * g, o);
+            for (int i = 0; i < 32; ++i) top = max3(top, __uint_as_float(x[0][i]), __uint_as_float(x[1][i]));
+          }
+          uint32_t packed[32];
+          float2 part[2];
+          while (true) {
+            const float shift = kLift - top * c;
+            const float2 shift2 = make_float2(shift, shift);
+            float peak[4] = {top, top, top, top};
+            part[0] = part[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float2 raw = make_float2(__uint_as_float(x[i / 16][2 * (i % 16)]), __uint_as_float(x[i / 16][2 * (i % 16) + 1]));
+              peak[i & 3] = max3(peak[i & 3], raw.x, raw.y);
+              float2 e = fma2(raw, c2, shift2);
+              e.x = exp2_approx(e.x);
+              e.y = exp2_approx(e.y);
+              part[i & 1] = add2(part[i & 1], e);
+              packed[i] = pack2<T>(e.x, e.y);
+            }
+            const float best = fmaxf(fmaxf(peak[0], peak[1]), fmaxf(peak[2], peak[3]));
+            if (!__any_sync(0xffffffffu, (best - top) * c > 8.0f)) break;
+            rare();
+            // O holds the products of all halves so far; the last one issued has to be complete
+            const bool issued = h == 1 || j > 0;
+            if (h == 1 && !wait.warp(half_done(s), tiles & 1, 8)) { alive = false; break; }
+            tcgen05_fence_after();
+            const float factor = exp2_approx((top - best) * c);
+            top = best;
+            sum *= factor;
+            if (issued) {
+#pragma unroll 1
+              for (int g = 0; g < HD / 32; ++g) {
+                uint32_t o[32];
+                tmem_load_32(o_addr + 32 * g, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                tmem_store_32(o_addr + 32 * g, o);
+              }
             }
           }
+          if (!alive) break;
+          part[0] = add2(part[0], part[1]);
+          sum += part[0].x + part[0].y;
+          tmem_store_32(s_addr + 32 * h, packed);
+          tmem_store_wait();
+          if (h == 0 && pending && !store()) { alive = false; break; }       // O is free for this unit's products
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(s, h));
         }
-        if (!alive) break;
-        part[0] = add2(part[0], part[1]);
-        sum += part[0].x + part[0].y;
-        tmem_store_32(s_addr + 32 * h, packed);
-        tmem_store_wait();
-        if (h == 0 && pending && !store()) { alive = false; break; }       // O is free for this unit's products
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(s, h));
       }
-    }
       if (alive && count) {
         pending = true;
         const int head = unit_of_round(round) % p.head_blocks * p.packed + thread % p.packed;
@@ -636,7 +636,6 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
         out_sum = sum;
       }
       t0 += (min(here.length, here.a + 2 * p.tile_tokens) + KEYS - 1) / KEYS;      // the tiles of both stages
-      if (count) release_v = last_stage ? (t0 - 1) % RING : -1;
     }
     if (alive && pending) store();
   }
