@@ -30,7 +30,7 @@ constexpr int kBadToken = 9;                           // device error code
 // ---- forward ---------------------------------------------------------------------------
 template <typename T> struct alignas(16) Vec { T v[16 / sizeof(T)]; };
 
-// 8 columns per thread: one or two 16-byte loads and stores.
+// 8 columns per thread: one or two 16-byte loads, one store of 16 or 32 bytes (which has to be aligned to its size).
 template <typename T> __device__ __forceinline__ void load8(float (&x)[8], const T* p) {
   constexpr int N = 16 / sizeof(T);
 #pragma unroll
@@ -453,6 +453,8 @@ __global__ void __launch_bounds__(256) embedding_gradient_kernel(GradientArgs a)
 
 bool known(int dtype) { return dtype == CT_F32 || dtype == CT_BF16 || dtype == CT_F16; }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// fp32 results leave in 32-byte stores, 16-bit ones in 16-byte stores
+bool stores_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (8 * dtype_size(dtype)) == 0; }
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t sort_blocks(int64_t tokens) { return tokens <= kClusterItems ? kCluster : (tokens + kManyItems - 1) / kManyItems; }
 int64_t piece_count(int64_t tokens) { return (tokens + kPiece - 1) / kPiece; }
@@ -542,7 +544,7 @@ extern "C" int ct_embedding_forward(const int64_t* ids, const void* table, void*
   int* flag = device_error_flag();
   if (!flag) return fail(CT_ERR_CUDA, "cannot allocate the device error flag");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool vector = width % 8 == 0 && aligned(table) && aligned(out);
+  const bool vector = width % 8 == 0 && aligned(table) && stores_aligned(out, out_dtype);
   const int64_t work = (tokens * (vector ? width / 8 : width) + 255) / 256;
   const unsigned grid = static_cast<unsigned>(work < (1 << 30) ? work : 1 << 30);
   return by_type(table_dtype, [&](auto w) {
@@ -598,7 +600,7 @@ extern "C" int ct_embedding_gradient(const void* dy, int64_t ld, const int64_t* 
     const int rc = sort_tokens(ids, tokens, rows, padding, keys, positions, other_keys, other_positions, histogram, flag, s);
     if (rc) return rc;
   }
-  const bool vector = width % 8 == 0 && aligned(dy) && aligned(d_table) && ld * dtype_size(dy_dtype) % 16 == 0;
+  const bool vector = width % 8 == 0 && aligned(dy) && stores_aligned(d_table, table_dtype) && ld * dtype_size(dy_dtype) % 16 == 0;
   return by_type(dy_dtype, [&](auto t) {
     return by_type(table_dtype, [&](auto w) {
       using T = decltype(t);

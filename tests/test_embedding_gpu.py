@@ -205,3 +205,24 @@ def test_refusals():
         embedding_gradient(dy[:3], ids, 10)
     with pytest.raises(ValueError, match="padding_idx"):
         embedding_gradient(dy, ids, 10, padding_idx=10)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+def test_results_at_any_element_of_a_buffer(dtype, offset):
+    """The C entries take results that begin anywhere: 16 bytes past a 32-byte boundary is too little for the widest store."""
+    tokens, rows, width = 37, 19, 24
+    weight, ids, dy = make_dy(rows, width, dtype), make_ids(tokens, rows, "uniform"), make_dy(tokens, width, dtype, seed=2)
+    library, code, stream = _lib.load(), _lib.code_of(TYPES[dtype]), _lib.stream_of(weight)
+    buffer = torch.full((64 + tokens * width,), 7.0, device="cuda", dtype=TYPES[dtype])
+    out = buffer[offset:offset + tokens * width]
+    _lib.check(library.ct_embedding_forward(ids.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens, rows, width, 1.0, code, code, stream))
+    assert torch.equal(out.view(tokens, width), weight[ids])
+    assert (buffer[:offset] == 7).all() and (buffer[offset + tokens * width:] == 7).all()
+    buffer.fill_(7.0)
+    table = buffer[offset:offset + rows * width]
+    workspace = torch.empty(library.ct_embedding_gradient_workspace(tokens, rows, width), device="cuda", dtype=torch.uint8)
+    _lib.check(library.ct_embedding_gradient(dy.data_ptr(), width, ids.data_ptr(), table.data_ptr(), tokens, rows, width, 1.0, -1, code, code,
+                                             workspace.data_ptr(), stream))
+    assert torch.equal(table.view(rows, width), embedding_gradient(dy, ids, rows, dtype=TYPES[dtype]))
+    assert (buffer[:offset] == 7).all() and (buffer[offset + rows * width:] == 7).all()
