@@ -1,6 +1,6 @@
 """Token embedding: lookup with scaling, and the table's gradient by sorted tokens.
 
-`embed_tokens` stands in for `nn.Embedding` and the cast of its result to the compute dtype (modeling/model.py:227
+`embed_tokens` stands in for the call of `nn.Embedding` and the cast of its result to the compute dtype (modeling/model.py:227
 of the reference; 185-193 for the embedding that trains). The lookup is one pass over the rows that are asked for. The
 gradient is a dense matrix, written once: tokens are sorted by id, every row of the table sums its tokens' gradients in
 token order, in fp32, without atomics, so repeated calls agree bit for bit.

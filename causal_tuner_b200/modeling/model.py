@@ -148,7 +148,7 @@ class Attention(nn.Module):
 
     def forward(self, x, cosine, sine, segments, spans, layout=None, *, residual=None):
         from ..kernels.attention import dense_attention, flash_dense
-        from ..kernels.attention_cuda import document_attention
+        from ..kernels.attention_cuda import document_attention, prepare_documents
         from ..kernels.linear import project_group
         b, s, _ = x.shape
         c, r = self.config, self.runtime
@@ -159,6 +159,8 @@ class Attention(nn.Module):
         if r.attention == "vanilla":
             y = dense_attention(q, k, v, segments)
         elif r.attention == "documents":
+            if layout is None:
+                layout = prepare_documents((b, s), spans, x.device, c.num_attention_heads, c.num_key_value_heads)
             y = document_attention(q, k, v, layout)
         else:
             y = flash_dense(q, k, v, spans, layout=layout)
@@ -182,11 +184,22 @@ class Layer(nn.Module):
         return self.mlp(normed, residual=shortcut, tile=mlp_tile, cache=mlp_cache)
 
 
+class TokenEmbedding(nn.Embedding):
+    """`nn.Embedding` whose decoder call, with the compute dtype, takes rows, factor and rounding in one kernel. A call of
+    the module, so that hooks on it run; without a dtype it is the base class's."""
+
+    def forward(self, ids, scale=1.0, dtype=None):
+        from ..kernels.embedding_cuda import embed_tokens
+        if dtype is None:
+            return super().forward(ids)
+        return embed_tokens(ids, self.weight, scale=scale, dtype=dtype, padding_idx=self.padding_idx)
+
+
 class Decoder(nn.Module):
     def __init__(self, config, runtime, device):
         super().__init__()
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, padding_idx=config.pad_token_id,
-                                         dtype=runtime.base_dtype, device=device)
+        self.embed_tokens = TokenEmbedding(config.vocab_size, config.hidden_size, padding_idx=config.pad_token_id,
+                                           dtype=runtime.base_dtype, device=device)
         self.layers = nn.ModuleList([Layer(config, runtime, device) for _ in range(config.num_hidden_layers)])
         self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps, runtime.base_dtype, device)
 
@@ -229,7 +242,6 @@ class CausalLM(nn.Module):
         from torch.utils.checkpoint import checkpoint
         from ..kernels.attention import prepare_dense_layout
         from ..kernels.attention_cuda import prepare_documents
-        from ..kernels.embedding_cuda import embed_tokens
         from ..segments import canonical_segments, position_ids, runs
         from .rotary import rotary_values
         r = self.runtime
@@ -241,9 +253,7 @@ class CausalLM(nn.Module):
             raise ValueError("position_ids exceed the model's logical position range")
         spans = batch.get("_spans") or runs(segments)
         cosine, sine = rotary_values(positions, self.config, r.compute_dtype)
-        table = self.model.embed_tokens
-        x = embed_tokens(batch["input_ids"], table.weight, scale=self.config.embed_scale, dtype=r.compute_dtype,
-                         padding_idx=table.padding_idx)
+        x = self.model.embed_tokens(batch["input_ids"], self.config.embed_scale, r.compute_dtype).to(r.compute_dtype)
         layout = None
         if r.attention == "flash_attention_2":
             layout = prepare_dense_layout(x.shape[:2], spans, x.device)

@@ -122,3 +122,39 @@ def test_updates_are_reproducible(golden):
     (first, values), (second, again) = run(), run()
     assert first == second and all(torch.equal(a, b) for a, b in zip(values, again))
     assert np.isfinite(first).all()
+
+
+def test_hooks_on_the_embedding_run(golden):
+    g = golden("step_tiny_b1.npz")
+    batch = {k: v.cuda() for k, v in batch_of(g).items()}
+    model = load_model(g, Runtime(rank=16, attention="documents", **FP32), nf4=False)
+    with torch.no_grad():
+        expected = model(batch)
+        seen = []
+        handle = model.model.embed_tokens.register_forward_hook(lambda module, args, out: seen.append(out.clone()) or 2 * out)
+        changed = model(batch)
+        handle.remove()
+        assert torch.equal(model(batch), expected) and not torch.equal(changed, expected)
+        table = model.model.embed_tokens
+        assert len(seen) == 1 and torch.equal(seen[0], table.weight[batch["input_ids"]])
+        assert torch.equal(table(batch["input_ids"]), seen[0])          # the module on its own
+
+
+def test_an_attention_block_without_a_prepared_layout(golden):
+    """As the library's form does, the block makes the plan from the spans it is given."""
+    from causal_tuner_b200.kernels.attention_cuda import prepare_documents
+    from causal_tuner_b200.modeling.rotary import rotary_values
+    from causal_tuner_b200.segments import canonical_segments, position_ids, runs
+    g = golden("step_tiny_b1.npz")
+    batch = {k: v.cuda() for k, v in batch_of(g).items()}
+    model = load_model(g, Runtime(rank=16, attention="documents", **FP32), nf4=False)
+    segments = canonical_segments(batch["attention_mask"], batch.get("segment_ids"))
+    spans, c = runs(segments), model.config
+    rotary = rotary_values(position_ids(segments), c, torch.float32)
+    with torch.no_grad():
+        x = model.model.embed_tokens(batch["input_ids"], 1.0, torch.float32)
+        block = model.model.layers[0].self_attn
+        plan = prepare_documents(x.shape[:2], spans, x.device, c.num_attention_heads, c.num_key_value_heads)
+        residual = torch.zeros_like(x)
+        results = [block(x, *rotary, segments, spans, layout, residual=residual) for layout in (None, plan)]
+    assert torch.equal(*results)
