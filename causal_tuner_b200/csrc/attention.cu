@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const PlanRe
   store_rows<T, HD>(out, static_cast<int64_t>(a.heads) * dim, acc, factor, row0, r.length, dim, ty, tx);
 }
 
-// The probabilities of one 64 x 64 tile and dS = P * (dP - delta), from s = q k^T and dp = dy v^T.
+// The probabilities of one 64 x 64 tile and dS = P * (dP - delta), from s = q k^T and dp = dy v^T. The document's first query
+// sees one key, so that P = 1, y = v and its dS is 0 (as a product with 0: a NaN stays one), not two sums' rounding errors.
 __device__ __forceinline__ void tile_slopes(float (&s)[4][4], float (&dp)[4][4], const float (&lse)[4], const float (&delta)[4],
                                             float scale, int row0, int key0, int length, int ty, int tx) {
 #pragma unroll
@@ -221,7 +222,7 @@ __device__ __forceinline__ void tile_slopes(float (&s)[4][4], float (&dp)[4][4],
       const int key = key0 + tx + 16 * j;
       const bool allowed = key <= row && row < length;
       s[i][j] = allowed ? exp2f(s[i][j] * scale - lse[i]) : 0.0f;
-      dp[i][j] = allowed ? s[i][j] * (dp[i][j] - delta[i]) : 0.0f;
+      dp[i][j] = allowed ? (row ? s[i][j] : 0.0f) * (dp[i][j] - delta[i]) : 0.0f;
     }
   }
 }

@@ -654,6 +654,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
 // dS is rounded to the operands' type for its two products, as P is for dv, and delta is formed in fp32 from the rounded
 // y: in bf16 dq and dk come out 2.4e-3 to 2.5e-3 (relative norm) from the exact values, 1.7e-3 of it the rounding of the
 // results themselves.
+// A document's first query sees one key: P = 1 and y = v, so its dS is 0 and is set to 0 (times 0: a NaN stays one); as
+// the difference of two sums it would be their rounding errors, and nothing but those for documents of one token.
 //
 // fp16 keeps 10 more bits of range for small probabilities: P is formed as 2^10 P (at most 1024) and the factor is
 // taken out of dv at the end and out of dS where it is formed.
@@ -933,6 +935,11 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_key_gradient_tc
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (32 * g + e < low || 32 * g + e >= high) x[e] = 0u;
+          if (token0 == 0 && key == 0) {                           // the document's first query
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * g + e < p.packed - 64 * half) x[e] = __float_as_uint(__uint_as_float(x[e]) * 0.0f);
+          }
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) packed[e] = pack2<T>(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
@@ -1196,15 +1203,19 @@ __global__ void __launch_bounds__(kBackwardThreads, 1) attention_query_gradient_
       const int token = w.here.a + thread / p.packed;
       return token < w.here.length ? (static_cast<int64_t>(w.here.start) + token) * p.heads + w.head0 + thread % p.packed : int64_t(-1);
     };
+    // infinite for the document's first query, which leaves nothing of its dS
+    auto log_sum = [&](const QueryWalk& w, int64_t row) {
+      return row < 0 ? 0.0f : w.here.a + thread / p.packed == 0 ? __int_as_float(0x7f800000) : p.lse[row];
+    };
     QueryWalk w(p);
     int64_t row = row_of(w);
-    float lse = row >= 0 ? p.lse[row] : 0.0f, delta = row >= 0 ? p.delta[row] : 0.0f;
+    float lse = log_sum(w, row), delta = row >= 0 ? p.delta[row] : 0.0f;
     while (w.valid() && alive) {
       const int last_key = min(w.here.a + thread / p.packed, w.here.length - 1);
       QueryWalk following = w;                                     // its statistics are on their way meanwhile
       following.next_unit();
       const int64_t next_row = following.valid() ? row_of(following) : int64_t(-1);
-      const float next_lse = next_row >= 0 ? p.lse[next_row] : 0.0f, next_delta = next_row >= 0 ? p.delta[next_row] : 0.0f;
+      const float next_lse = log_sum(following, next_row), next_delta = next_row >= 0 ? p.delta[next_row] : 0.0f;
       for (int j = 0; j < w.n; ++j, ++t) {
         const int all_cols = w.both_halves(j) ? KEYS : 64;
         const bool idle = half && all_cols == 64;                  // nothing in this warpgroup's 64 columns

@@ -12,6 +12,9 @@ Bounds, for a type with rounding error u (half a step, torch.finfo(t).eps / 2) a
                 and of the output, which are kept 2^10 and 2^7 above their size
                 the 16-bit path's exponentials flush results below 2^-126 to zero, or (those on the FMA units) hold them at
                 2^-125: an absolute step of 2^-125 per probability, times what it multiplies
+                for dS that is the computed dP - delta: with d' = d + x, |P'd' - Pd| <= |P' - P| |d| + P'|x|, and
+                P' <= (1 + w + r) P + 2^-125, so the error x of the difference counts with P + 2^-125, not with P alone
+                (seen where a key's probabilities all vanish and d is smaller than x)
   dv, dq, dk    the same sums over absolute values, times 1 + (terms) e, plus u of the result
 """
 
@@ -53,7 +56,7 @@ def reference(q, k, v, spans, scale, dy=None, rounded=True):
             delta_error = (g.abs() * (y_error + dim * e * y.abs())).sum(-1, keepdim=True)
             slope = p * (dp - delta)
             seen = allowed.double()
-            slope_error = (w + r) * slope.abs() + (t + f * (dp - delta).abs()) * seen + p * (dim * e * (g.abs() @ vd.abs().T) + delta_error)
+            slope_error = (w + r) * slope.abs() + (t + f * (dp - delta).abs()) * seen + (p + f * seen) * (dim * e * (g.abs() @ vd.abs().T) + delta_error)
             values["dv"][row, start:end, s] += p.T @ g
             errors["dv"][row, start:end, s] += (((w + r) * p + (t * 2 ** -10 + f) * seen).T @ g.abs()) * terms + (n * group) * e * (p.T @ g.abs())
             values["dq"][row, start:end, h] = slope @ kd * scale

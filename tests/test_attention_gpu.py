@@ -372,3 +372,21 @@ def test_refusals():
         attention_backward(dy, q, k, v, y, lse[:5], plan)
     with pytest.raises(ValueError, match="on one device"):
         document_attention(q, k, v, prepare_documents((2, 20), ((0, 0, 20),), "cpu", 4))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("heads, kv_heads", [(4, 1), (3, 3), (256, 1)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_first_query_of_a_document_has_no_score_gradient(dtype, heads, kv_heads, dim):
+    """It sees one key: P = 1 whatever its score, so dq is 0 for it, and dq and dk are for documents of one token."""
+    q, k, v, dy = tensors(2, 150, heads, kv_heads, dim, dtype, factor=8.0)
+    spans = ((0, 0, 1), (0, 1, 2), (0, 5, 140), (0, 140, 150), (1, 3, 4), (1, 4, 149), (1, 149, 150))
+    grads = check(q, k, v, dy, spans)
+    for row, start, end in spans:
+        assert (grads["dq"][row, start] == 0).all()
+        if end - start == 1:
+            assert (grads["dk"][row, start] == 0).all() and (grads["dv"][row, start] != 0).any()
+    dy[0, 1, 0, 0] = float("nan")                            # no zero hides it
+    grads = run(q, k, v, dy, spans)
+    assert torch.isnan(grads["dq"][0, 1, 0]).all() and torch.isnan(grads["dk"][0, 1, 0]).all() and torch.isnan(grads["dv"][0, 1, 0, 0])
+    assert (grads["dq"][0, 1, 1:] == 0).all() and (grads["dq"][0, 0] == 0).all()
