@@ -649,8 +649,8 @@ __global__ void __launch_bounds__(kForwardThreads, 1) attention_forward_tc_kerne
 // ---- backward ------------------------------------------------------------------------
 // Two kernels that each recompute the probabilities, instead of one that would have to add query gradients from many key
 // tiles into memory: 14 instead of 10 FLOP per pair and channel, but no atomics and no order that changes the sums.
-// Measured, 4 x 4096 tokens, 32 heads of 128 on one key head, bf16: query gradients 640 us, key gradients 928 us, delta
-// 48 us, sum of the pieces 16 us (1225 TFLOP/s of the products that run; FlashAttention-2 with atomics: 4.5 ms).
+// Measured, 4 x 4096 tokens, 32 heads of 128 on one key head, bf16: query gradients 653 us, key gradients 954 us, delta
+// 48 us, sum of the pieces 16 us (1196 TFLOP/s of the products that run; FlashAttention-2 with atomics: 4.5 ms).
 // dS is rounded to the operands' type for its two products, as P is for dv, and delta is formed in fp32 from the rounded
 // y: in bf16 dq and dk come out 2.4e-3 to 2.5e-3 (relative norm) from the exact values, 1.7e-3 of it the rounding of the
 // results themselves.
